@@ -98,6 +98,8 @@ def _bind_native(L: ctypes.CDLL):
     f.bind(addr(L.candle_moe_apply_topk_softmax_inplace), addr(L.candle_moe_fused_moe_forward),
            addr(L.candle_moe_router_topk), addr(L.candle_moe_fused_moe_fp8), addr(L.candle_moe_fused_moe_packed),
            raw_stream)
+    f.bind_ops(addr(L.candle_moe_topk_route), addr(L.candle_moe_add_rms_norm), addr(L.candle_moe_fused_moe_mxfp4),
+               torch._C._cuda_getDevice)
     return f
 
 
@@ -164,6 +166,17 @@ def lib() -> ctypes.CDLL:
         L.candle_moe_grouping_workspace_size.restype = sz
         L.candle_moe_group_pairs.argtypes = [vp, i32, i32, vp, vp, vp, sz, vp]
         L.candle_moe_group_pairs.restype = i32
+        f32 = ctypes.c_float
+        L.candle_moe_topk_route.argtypes = [vp, u32, vp, vp, vp, vp] + [i32] * 8 + [f32, vp]
+        L.candle_moe_topk_route.restype = i32
+        L.candle_moe_add_rms_norm.argtypes = [vp] * 7 + [i32, i32, f32, u32, vp]
+        L.candle_moe_add_rms_norm.restype = i32
+        L.candle_moe_quantize_mxfp4.argtypes = [vp, u32, i32, i32, i32, i32, vp, vp, vp]
+        L.candle_moe_quantize_mxfp4.restype = i32
+        L.candle_moe_dequantize_mxfp4.argtypes = [vp, vp, i32, i32, i32, vp, u32, vp]
+        L.candle_moe_dequantize_mxfp4.restype = i32
+        L.candle_moe_fused_moe_mxfp4.argtypes = [vp] * 11 + [i32] * 6 + [u32, u32, i32, vp]
+        L.candle_moe_fused_moe_mxfp4.restype = i32
         L.candle_moe_trim_workspaces.argtypes = []
         L.candle_moe_trim_workspaces.restype = i32
         L.candle_moe_last_error.argtypes = []
@@ -504,6 +517,198 @@ def fused_moe_packed(input, gate_packed, up_packed, down_packed, routing_weights
         T, H, I, num_experts, top_k, int(activation), int(moe_type), _torch_dtype_code(input), _stream_for(input)))
 
 
+def _ptr(t):
+    return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+
+def _require(who: str, device, want) -> None:
+    """Each (name, tensor, shape, dtypes): contiguous, on `device`, of this shape and one of these dtypes."""
+    for name, t, shape, dtypes in want:
+        problem = None
+        if t is None:
+            problem = "is missing"
+        elif tuple(t.shape) != tuple(shape):
+            problem = f"must be {list(shape)}, got {list(t.shape)}"
+        elif t.dtype not in dtypes:
+            problem = f"must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}"
+        elif not t.is_contiguous():
+            problem = "must be contiguous"
+        elif t.device != device:
+            problem = f"must be on {device}, got {t.device}"
+        if problem:
+            raise CandleMoeError(CANDLE_MOE_ERR_INVALID, f"{who}: {name} {problem}")
+
+
+def _launch_on(t, who: str, call) -> None:
+    """check(call(stream)) with t's device current and its current stream."""
+    import torch
+
+    if not t.is_cuda:
+        raise CandleMoeError(CANDLE_MOE_ERR_INVALID, f"{who}: tensors must be on the GPU, got {t.device}")
+    with torch.cuda.device(t.device):
+        check(call(_stream_for(t)))
+
+
+SCORE_CODES = {"softmax": 0, "sigmoid": 1}
+
+
+def topk_route(logits, topk_weight, topk_indices, token_expert_indices, bias=None, score: str = "softmax",
+               num_groups: int = 1, topk_groups: int = 1, group_top: int = 1, renormalize: bool = True,
+               scale: float = 1.0) -> None:
+    """Routing with groups, written in place (candle_moe_topk_route).
+
+    logits [T, E] f32, f16 or bf16; bias [E] f32 or None. The experts' scores s
+    are the softmax ("softmax") or the logistic function ("sigmoid") of the
+    logits; the choice goes by c = s + bias: of num_groups groups of neighbouring
+    experts the topk_groups with the largest sums of their group_top (1 or 2) best
+    c, and in those the k best c, ties to the lower index. topk_weight [T, k] f32 = s of the
+    chosen, divided by their sum with renormalize, times scale; topk_indices and
+    token_expert_indices [T, k] u32 (int32 accepted) as apply_topk_softmax_inplace's."""
+    code = SCORE_CODES.get(score)
+    if code is None:
+        raise CandleMoeError(CANDLE_MOE_ERR_INVALID, f"topk_route: score must be softmax or sigmoid, got {score!r}")
+    if _native is not None:
+        rc = _native.route(logits, bias, topk_weight, topk_indices, token_expert_indices, code, num_groups, topk_groups,
+                           group_top, renormalize, scale)
+        if rc is not None:
+            return check(rc)
+    import torch
+
+    if logits.dim() != 2 or topk_weight.dim() != 2:
+        raise CandleMoeError(CANDLE_MOE_ERR_INVALID, "topk_route: logits must be [T, E] and topk_weight [T, k]")
+    T, E = logits.shape
+    tk = (T, topk_weight.shape[1])
+    index = (torch.int32, torch.uint32)
+    want = [("logits", logits, (T, E), (torch.float32, torch.float16, torch.bfloat16)),
+            ("topk_weight", topk_weight, tk, (torch.float32,)), ("topk_indices", topk_indices, tk, index),
+            ("token_expert_indices", token_expert_indices, tk, index)]
+    if bias is not None:
+        want.append(("bias", bias, (E,), (torch.float32,)))
+    _require("topk_route", logits.device, want)
+    _launch_on(logits, "topk_route", lambda s: lib().candle_moe_topk_route(
+        _ptr(logits), _torch_dtype_code(logits), _ptr(bias), _ptr(topk_weight), _ptr(topk_indices),
+        _ptr(token_expert_indices), E, T, tk[1], code, int(num_groups), int(topk_groups), int(group_top),
+        1 if renormalize else 0, float(scale), s))
+
+
+def add_rms_norm(input, weight, eps: float, residual=None, residual_output=None, output=None, codes=None,
+                 scales=None) -> None:
+    """The residual's addition and the root-mean-square norm, written in place
+    (candle_moe_add_rms_norm): z = input + residual (input without one),
+    residual_output = z, output = y = z / sqrt(mean(z^2) + eps) * weight of z before
+    its rounding, and codes [T, H] uint8 with scales [T, H / 32] uint8: y as MXFP8
+    (e4m3 values, one power of two per 32), the 8-bit rows fused_moe_mxfp4 takes.
+    input, residual, residual_output, output [T, H] and weight [H] f32, f16 or bf16.
+    Any output may be None, but one of output and codes is needed; residual_output
+    may be residual. With codes H is a multiple of 32."""
+    if _native is not None:
+        rc = _native.norm(input, weight, eps, residual, residual_output, output, codes, scales)
+        if rc is not None:
+            return check(rc)
+    import torch
+
+    if input.dim() != 2:
+        raise CandleMoeError(CANDLE_MOE_ERR_INVALID, "add_rms_norm: input must be [T, H]")
+    T, H = input.shape
+    same = (input.dtype,)
+    want = [("input", input, (T, H), (torch.float32, torch.float16, torch.bfloat16)), ("weight", weight, (H,), same)]
+    want += [(n, t, (T, H), same) for n, t in (("residual", residual), ("residual_output", residual_output),
+                                               ("output", output)) if t is not None]
+    if codes is not None or scales is not None:
+        want += [("codes", codes, (T, H), (torch.uint8,)), ("scales", scales, (T, H // 32), (torch.uint8,))]
+    _require("add_rms_norm", input.device, want)
+    _launch_on(input, "add_rms_norm", lambda s: lib().candle_moe_add_rms_norm(
+        _ptr(input), _ptr(residual), _ptr(weight), _ptr(residual_output), _ptr(output), _ptr(codes), _ptr(scales), T, H,
+        float(eps), _torch_dtype_code(input), s))
+
+
+def quantize_mxfp4(weights, input_kn: bool = True):
+    """4-bit form of expert weights (candle_moe_quantize_mxfp4): weights [E, K, N]
+    (input_kn) or [E, N, K], f32/f16/bf16, contiguous, on the GPU, K a multiple of 32
+    -> (codes [E, N, K / 2] uint8, scales [E, N, K / 32] uint8), e2m1 values and one
+    power of two per 32 along K."""
+    import torch
+
+    if weights.dim() != 3 or not weights.is_contiguous():
+        raise CandleMoeError(CANDLE_MOE_ERR_INVALID, "quantize_mxfp4: weights must be contiguous [E, K, N] or [E, N, K]")
+    E = weights.shape[0]
+    K, N = (weights.shape[1], weights.shape[2]) if input_kn else (weights.shape[2], weights.shape[1])
+    code = _torch_dtype_code(weights)
+    codes = torch.empty((E, N, K // 2), dtype=torch.uint8, device=weights.device)
+    scales = torch.empty((E, N, K // 32), dtype=torch.uint8, device=weights.device)
+    _launch_on(weights, "quantize_mxfp4", lambda s: lib().candle_moe_quantize_mxfp4(
+        _ptr(weights), code, E, K, N, 1 if input_kn else 0, _ptr(codes), _ptr(scales), s))
+    return codes, scales
+
+
+def dequantize_mxfp4(codes, scales, dtype):
+    """The [E, N, K] weights of torch dtype that MXFP4 codes [E, N, K / 2] and
+    scales [E, N, K / 32] stand for (candle_moe_dequantize_mxfp4)."""
+    import torch
+
+    if codes.dim() != 3:
+        raise CandleMoeError(CANDLE_MOE_ERR_INVALID, "dequantize_mxfp4: codes must be [E, N, K / 2]")
+    E, N, K = codes.shape[0], codes.shape[1], codes.shape[2] * 2
+    _require("dequantize_mxfp4", codes.device, [("codes", codes, (E, N, K // 2), (torch.uint8,)),
+                                                ("scales", scales, (E, N, K // 32), (torch.uint8,))])
+    out = torch.empty((E, N, K), dtype=dtype, device=codes.device)
+    code = _torch_dtype_code(out)
+    _launch_on(codes, "dequantize_mxfp4", lambda s: lib().candle_moe_dequantize_mxfp4(
+        _ptr(codes), _ptr(scales), E, N, K, _ptr(out), code, s))
+    return out
+
+
+def fused_moe_mxfp4(input, gate_q, up_q, down_q, gate_scale, up_scale, down_scale, routing_weights, expert_indices,
+                    output, num_experts: int, top_k: int, activation: int = 0, moe_type: int = 0, input_scale=None,
+                    accumulate: bool = True) -> None:
+    """output += (accumulate) or = the MoE of input over 4-bit expert weights
+    (candle_moe_fused_moe_mxfp4). Qwen3 (moe_type 0): gate_q / up_q codes
+    [E, I, H / 2] uint8 with scales [E, I, H / 32] uint8, down_q [E, H, I / 2] with
+    [E, H, I / 32] (quantize_mxfp4 of the API layout); Nomic (moe_type 1): gate_q =
+    fc1 like gate, up_q = fc2 like down (input_kn False), down_q and down_scale None.
+    output [T, H] f16 or bf16; input [T, H] of output's dtype, or with input_scale
+    [T, H / 32] uint8 the 8-bit rows of add_rms_norm (uint8). routing_weights [T, k]
+    f32, expert_indices [T, k] u32/i32 (ids >= E: dropped). Every tensor contiguous
+    and on input's device, H and I multiples of 32."""
+    if _native is not None:
+        rc = _native.mxfp4(input, gate_q, up_q, down_q, gate_scale, up_scale, down_scale, routing_weights,
+                           expert_indices, output, num_experts, top_k, activation, moe_type, input_scale, accumulate)
+        if rc is not None:
+            return check(rc)
+    import torch
+
+    def bad(msg):
+        raise CandleMoeError(CANDLE_MOE_ERR_INVALID, "fused_moe_mxfp4: " + msg)
+
+    if input.dim() != 2 or gate_q.dim() != 3:
+        bad("input must be [T, H] and gate_q [E, I, H / 2]")
+    (T, H), E, I = input.shape, num_experts, gate_q.shape[1]
+    u8, qwen3 = (torch.uint8,), moe_type == 0
+    if H % 32 or I % 32:
+        raise CandleMoeError(CANDLE_MOE_ERR_UNSUPPORTED, "fused_moe_mxfp4: hidden_dim and intermediate_dim must be "
+                             f"positive multiples of 32 (got {H}, {I})")
+    first, last = ((E, I, H // 2), (E, I, H // 32)), ((E, H, I // 2), (E, H, I // 32))
+    second = first if qwen3 else last
+    want = [("output", output, (T, H), (torch.float16, torch.bfloat16)),
+            ("gate_q", gate_q, first[0], u8), ("gate_scale", gate_scale, first[1], u8),
+            ("up_q", up_q, second[0], u8), ("up_scale", up_scale, second[1], u8)]
+    if qwen3:
+        want += [("down_q", down_q, last[0], u8), ("down_scale", down_scale, last[1], u8)]
+    elif down_q is not None or down_scale is not None:
+        bad("Nomic (moe_type 1) takes no down_q / down_scale")
+    want += [("routing_weights", routing_weights, (T, top_k), (torch.float32,)),
+             ("expert_indices", expert_indices, (T, top_k), (torch.int32, torch.uint32))]
+    if input_scale is not None:
+        want += [("input", input, (T, H), u8), ("input_scale", input_scale, (T, H // 32), u8)]
+    else:
+        want.append(("input", input, (T, H), () if output is None else (output.dtype,)))
+    _require("fused_moe_mxfp4", input.device, want)
+    _launch_on(input, "fused_moe_mxfp4", lambda s: lib().candle_moe_fused_moe_mxfp4(
+        _ptr(input), _ptr(input_scale), _ptr(gate_q), _ptr(up_q), _ptr(down_q), _ptr(gate_scale), _ptr(up_scale),
+        _ptr(down_scale), _ptr(routing_weights), _ptr(expert_indices), _ptr(output), T, H, I, E, int(top_k),
+        int(activation), int(moe_type), _torch_dtype_code(output), 1 if accumulate else 0, s))
+
+
 def validate_topk_softmax(g: CmTensor, w: CmTensor, i: CmTensor, ei: CmTensor) -> None:
     check(lib().candle_moe_validate_topk_softmax(ctypes.byref(g), ctypes.byref(w), ctypes.byref(i), ctypes.byref(ei)))
 
@@ -644,4 +849,5 @@ __all__ = [
     "Activation", "FusedMoE", "apply_topk_softmax_inplace", "CandleMoeError", "lib", "describe", "spec",
     "validate_topk_softmax", "version", "LIB_PATH", "set_combine_policy", "fused_moe_path",
     "set_tile_policy", "fused_moe_tile", "fused_moe_kernel", "quantize_fp8", "dequantize_fp8", "fused_moe_fp8",
+    "topk_route", "add_rms_norm", "quantize_mxfp4", "dequantize_mxfp4", "fused_moe_mxfp4",
 ]

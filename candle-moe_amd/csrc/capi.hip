@@ -48,7 +48,7 @@ int set_error(int code, const char* fmt, ...) {
 
 void clear_error() { g_last_error.clear(); }
 
-static int hip_fail(hipError_t e, const char* what) {
+int hip_fail(hipError_t e, const char* what) {
     return set_error(CANDLE_MOE_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
@@ -1212,6 +1212,24 @@ static int ws_fail(const char* who, size_t need, hipError_t e) {
                          "the %zu bytes this call needs: make one call of this size on the stream before capturing",
                          who, need);
     return set_error(CANDLE_MOE_ERR_WORKSPACE, "%s: hipMallocAsync(%zu) failed: %s", who, need, hipGetErrorString(e));
+}
+
+int lease_workspace(const char* who, size_t need, size_t reserve, hipStream_t s, WsLease& l) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return hip_fail(e, who);
+    l.lock = std::unique_lock<std::mutex>(g_ws_mu);
+    OwnedWs* w = owned_ws_locked(dev, s, need, std::max(need, reserve), e);
+    if (!w) return ws_fail(who, need, e);
+    l.ptr = static_cast<char*>(w->ptr);
+    l.bytes = w->bytes;
+    return CANDLE_MOE_OK;
+}
+
+size_t packed_upto_bytes(int T, int H, int I, int E, int k, int act, uint32_t moe_type, uint32_t dtype) {
+    Problem p;
+    if (check_problem(T, H, I, E, k, act, moe_type, dtype, p, true, true, false, true)) return 0;
+    return upto_bytes(p);
 }
 
 int trim_owned_workspaces() {

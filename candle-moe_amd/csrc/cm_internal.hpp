@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <mutex>
+
 namespace cm {
 
 // ---------------------------------------------------------------- router
@@ -26,6 +28,38 @@ hipError_t launch_topk_softmax(const void* logits, int in_dtype, void* w, int w_
                                uint32_t* ei, int T, int E, int k, hipStream_t stream);
 // test support: the router's f32 exponential against its f64 one
 hipError_t launch_router_exp_check(uint32_t first, uint32_t n, uint32_t* stats, hipStream_t stream);
+
+// Routing with groups (route.hip): dtype of the logits, score kRouteSoftmax or
+// kRouteSigmoid; idx, w and ei [T, k].
+enum RouteScore : int { kRouteSoftmax = 0, kRouteSigmoid = 1 };
+constexpr int kRouteMaxGroups = 64;
+struct RouteArgs {
+    const void* logits;
+    const float* bias;  // [E] or null
+    float* w;
+    uint32_t* idx;
+    uint32_t* ei;
+    int T, E, k, dtype, score, groups, topk_groups, group_top, renorm;
+    float scale;
+};
+hipError_t launch_route(const RouteArgs& a, hipStream_t stream);
+
+// ------------------------------------------------------------------ norm
+// rms_norm.hip. x, residual (or null), weight [H], residual_out (or null), out
+// (or null) of one dtype; codes, scales (or null, H a multiple of 32). vec: H is
+// a multiple of 8 and every pointer is 16-byte aligned.
+struct NormArgs {
+    const void* x;
+    const void* residual;
+    const void* weight;
+    void* residual_out;
+    void* out;
+    uint8_t* codes;
+    uint8_t* scales;
+    int T, H, vec;
+    float eps;
+};
+hipError_t launch_add_rms_norm(const NormArgs& a, int dtype, hipStream_t stream);
 
 // -------------------------------------------------------------- grouping
 // Pairs p = t*k + j are grouped by expert idx[p] (stable: ascending p inside
@@ -342,6 +376,15 @@ hipError_t launch_dequantize_fp8(const uint8_t* q, const float* scales, int E, i
 // 16-bit weights [E][K][N] -> K-contiguous [E][N][K] (the pre-packed format)
 hipError_t launch_pack_kn(const void* w, int E, int K, int N, void* out, hipStream_t stream);
 
+// 4-bit weights (mxfp4.hip): codes [E][N][K/2], scales [E][N][K/32], K a
+// multiple of 32; MXFP8 rows [T][H], scales [T][H/32] to a 16-bit dtype
+hipError_t launch_quantize_mxfp4(const void* w, int dtype, int E, int K, int N, int kn, uint8_t* codes,
+                                 uint8_t* scales, hipStream_t stream);
+hipError_t launch_dequantize_mxfp4(const void* codes, const void* scales, int E, int N, int K, void* out, int dtype,
+                                   hipStream_t stream);
+hipError_t launch_rows8_to(const void* codes, const void* scales, long long T, int H, void* out, int dtype,
+                           hipStream_t stream);
+
 // f32 accumulator helpers
 hipError_t launch_fill_zero_f32(float* p, long long n, hipStream_t stream);
 hipError_t launch_fill_zero_bytes(void* p, long long nbytes, hipStream_t stream);
@@ -357,6 +400,18 @@ hipError_t launch_finalize(void* out, int dtype, const float* acc, long long n, 
 // Record the message of a failing call (thread-local) and return `code`.
 int set_error(int code, const char* fmt, ...);
 void clear_error();
+int hip_fail(hipError_t e, const char* what);
+// The library-owned workspace of (current device, s), held until `lock` goes.
+// need: bytes a call takes; reserve (>= need): bytes to have for the calls to come.
+struct WsLease {
+    std::unique_lock<std::mutex> lock;
+    char* ptr = nullptr;
+    size_t bytes = 0;
+};
+int lease_workspace(const char* who, size_t need, size_t reserve, hipStream_t s, WsLease& l);
+// Workspace of fused_moe over pre-packed 16-bit weights for every batch up to T
+// tokens (aligned operands); 0 with the error set where the sizes are refused.
+size_t packed_upto_bytes(int T, int H, int I, int E, int k, int act, uint32_t moe_type, uint32_t dtype);
 int topk_softmax_impl(const void* g, int gdt, void* w, int wdt, void* idx, void* ei, int E, int T, int k,
                       void* stream);
 struct Fp8Weights;

@@ -31,6 +31,11 @@ decltype(&candle_moe_router_topk) g_router;
 decltype(&candle_moe_fused_moe_fp8) g_fp8;
 decltype(&candle_moe_fused_moe_packed) g_packed;
 PyObject* g_raw_stream;  // torch._C._cuda_getCurrentRawStream
+// (bind_ops())
+decltype(&candle_moe_topk_route) g_route;
+decltype(&candle_moe_add_rms_norm) g_norm;
+decltype(&candle_moe_fused_moe_mxfp4) g_mxfp4;
+PyObject* g_device;  // torch._C._cuda_getDevice
 
 int dtype_code(at::ScalarType t) {
     switch (t) {
@@ -292,9 +297,169 @@ PyObject* prepared(PyObject* const* a, Py_ssize_t n, bool fp8) {
 PyObject* py_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) { return prepared(a, n, true); }
 PyObject* py_packed(PyObject*, PyObject* const* a, Py_ssize_t n) { return prepared(a, n, false); }
 
+// bind_ops(route, norm, mxfp4, get_device): entry point addresses
+PyObject* py_bind_ops(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (!argc(n, 4)) return nullptr;
+    void* p[3];
+    for (int i = 0; i < 3; ++i) {
+        p[i] = PyLong_AsVoidPtr(a[i]);
+        if (PyErr_Occurred()) return nullptr;
+    }
+    g_route = reinterpret_cast<decltype(g_route)>(p[0]);
+    g_norm = reinterpret_cast<decltype(g_norm)>(p[1]);
+    g_mxfp4 = reinterpret_cast<decltype(g_mxfp4)>(p[2]);
+    Py_INCREF(a[3]);
+    Py_XSETREF(g_device, a[3]);
+    Py_RETURN_NONE;
+}
+
+// The current stream of t's device, which has to be the current one; 0: it is
+// not (the general route makes it current), -1: a Python error is set.
+int stream_here(const at::Tensor& t, void** s) {
+    PyObject* r = PyObject_CallNoArgs(g_device);
+    if (!r) return -1;
+    const long dev = PyLong_AsLong(r);
+    Py_DECREF(r);
+    if (dev == -1 && PyErr_Occurred()) return -1;
+    if (dev != t.get_device()) return 0;
+    return stream_of(t, s) ? 1 : -1;
+}
+
+bool is_float(const at::Tensor* t) {
+    const at::ScalarType ty = t->scalar_type();
+    return ty == at::kHalf || ty == at::kBFloat16 || ty == at::kFloat;
+}
+// a bool or int as 0 / 1, a float or int as double; false where it is something else
+bool flag(PyObject* o, int* v) {
+    if (!PyBool_Check(o) && !PyLong_Check(o)) return false;
+    *v = PyObject_IsTrue(o);
+    return *v >= 0;
+}
+bool number(PyObject* o, double* v) {
+    if (!PyFloat_Check(o)) return false;
+    *v = PyFloat_AS_DOUBLE(o);
+    return true;
+}
+
+// route(logits, bias or None, weight, indices, token_expert_indices, score,
+// num_groups, topk_groups, group_top, renormalize, scale) -> status or None
+PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (!argc(n, 11)) return nullptr;
+        long long v[4];
+        int renorm;
+        double scale;
+        if (!ints(a + 5, 4, v) || !flag(a[9], &renorm) || !number(a[10], &scale)) Py_RETURN_NONE;
+        for (long long x : v)
+            if (x < 0 || x > INT_MAX) Py_RETURN_NONE;
+        const at::Tensor *l = plain(a[0]), *b = a[1] == Py_None ? nullptr : plain(a[1]);
+        const at::Tensor *w = plain(a[2]), *i = plain(a[3]), *ei = plain(a[4]);
+        if (!l || !w || !i || !ei || (!b && a[1] != Py_None)) Py_RETURN_NONE;
+        if (!l->is_cuda() || l->dim() != 2 || w->dim() != 2 || !is_float(l) || !l->is_contiguous()) Py_RETURN_NONE;
+        const int64_t T = l->size(0), E = l->size(1), k = w->size(1), tk[2] = {T, k};
+        const at::Device dev = l->device();
+        if (T > INT_MAX || E > INT_MAX || k > INT_MAX || !is(w, at::kFloat, dev, tk) || !is_index(i, dev, tk) ||
+            !is_index(ei, dev, tk) || (b && !is(b, at::kFloat, dev, {E})))
+            Py_RETURN_NONE;
+        void* s;
+        const int here = stream_here(*l, &s);
+        if (here < 0) return nullptr;
+        if (here == 0) Py_RETURN_NONE;
+        const void *lp = l->data_ptr(), *bp = b ? b->data_ptr() : nullptr;
+        void *wp = w->data_ptr(), *ip = i->data_ptr(), *ep = ei->data_ptr();
+        const uint32_t code = (uint32_t)dtype_code(l->scalar_type());
+        return call([&] {
+            return g_route(lp, code, static_cast<const float*>(bp), static_cast<float*>(wp), ip, ep, (int)E, (int)T,
+                           (int)k, (int)v[0], (int)v[1], (int)v[2], (int)v[3], renorm, (float)scale, s);
+        });
+    });
+}
+
+// norm(input, weight, eps, residual, residual_output, output, codes, scales),
+// the last five or None -> status or None
+PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (!argc(n, 8)) return nullptr;
+        double eps;
+        if (!number(a[2], &eps)) Py_RETURN_NONE;
+        const at::Tensor *x = plain(a[0]), *w = plain(a[1]), *o[5];
+        for (int i = 0; i < 5; ++i) {
+            o[i] = a[3 + i] == Py_None ? nullptr : plain(a[3 + i]);
+            if (!o[i] && a[3 + i] != Py_None) Py_RETURN_NONE;
+        }
+        if (!x || !w || !x->is_cuda() || x->dim() != 2 || !is_float(x) || !x->is_contiguous()) Py_RETURN_NONE;
+        const int64_t T = x->size(0), H = x->size(1), th[2] = {T, H}, ts[2] = {T, H / 32};
+        const at::Device dev = x->device();
+        const at::ScalarType ty = x->scalar_type();
+        if (T > INT_MAX || H > INT_MAX || !is(w, ty, dev, {H})) Py_RETURN_NONE;
+        for (int i = 0; i < 3; ++i)
+            if (o[i] && !is(o[i], ty, dev, th)) Py_RETURN_NONE;
+        if (!o[3] != !o[4] || (o[3] && (!is(o[3], at::kByte, dev, th) || !is(o[4], at::kByte, dev, ts)))) Py_RETURN_NONE;
+        void* s;
+        const int here = stream_here(*x, &s);
+        if (here < 0) return nullptr;
+        if (here == 0) Py_RETURN_NONE;
+        void* p[5];
+        for (int i = 0; i < 5; ++i) p[i] = o[i] ? o[i]->data_ptr() : nullptr;
+        const void *xp = x->data_ptr(), *wp = w->data_ptr();
+        const uint32_t code = (uint32_t)dtype_code(ty);
+        return call([&] { return g_norm(xp, p[0], wp, p[1], p[2], p[3], p[4], (int)T, (int)H, (float)eps, code, s); });
+    });
+}
+
+// mxfp4(input, gate, up, down or None, their scales, weights, indices, output,
+// E, k, act, moe_type, input_scale or None, accumulate) -> status or None
+PyObject* py_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (!argc(n, 16)) return nullptr;
+        long long v[4];
+        int acc;
+        if (!ints(a + 10, 4, v) || !flag(a[15], &acc)) Py_RETURN_NONE;
+        const long long E = v[0], k = v[1];
+        if (v[3] < 0 || v[3] > 1 || v[2] < 0 || v[2] > 2 || E < 1 || k < 1 || E > INT_MAX || k > INT_MAX)
+            Py_RETURN_NONE;
+        const bool qwen3 = v[3] == 0;
+        const at::Tensor* t[11];  // input, gate, up, down, scales, weights, indices, output; then input_scale
+        for (int i = 0; i < 11; ++i) {
+            PyObject* o = a[i < 10 ? i : 14];
+            t[i] = o == Py_None ? nullptr : plain(o);
+            if (!t[i] && o != Py_None) Py_RETURN_NONE;
+        }
+        const at::Tensor *x = t[0], *gate = t[1], *out = t[9];
+        if (!x || !gate || !out || !x->is_cuda() || x->dim() != 2 || gate->dim() != 3 || !x->is_contiguous() ||
+            (out->scalar_type() != at::kHalf && out->scalar_type() != at::kBFloat16))
+            Py_RETURN_NONE;
+        const int64_t T = x->size(0), H = x->size(1), I = gate->size(1);
+        if (T > INT_MAX || H > INT_MAX || I > INT_MAX || H % 32 || I % 32) Py_RETURN_NONE;
+        const at::Device dev = x->device();
+        const at::ScalarType ty = out->scalar_type();
+        const int64_t q1[3] = {E, I, H / 2}, s1[3] = {E, I, H / 32}, q2[3] = {E, H, I / 2}, s2[3] = {E, H, I / 32};
+        const int64_t tk[2] = {T, k}, th[2] = {T, H}, ts[2] = {T, H / 32};
+        if (x->scalar_type() != (t[10] ? at::kByte : ty) || (t[10] && !is(t[10], at::kByte, dev, ts)) ||
+            !is(out, ty, dev, th) || !is(gate, at::kByte, dev, q1) || !is(t[4], at::kByte, dev, s1) ||
+            !is(t[2], at::kByte, dev, qwen3 ? at::IntArrayRef(q1) : at::IntArrayRef(q2)) ||
+            !is(t[5], at::kByte, dev, qwen3 ? at::IntArrayRef(s1) : at::IntArrayRef(s2)) ||
+            (qwen3 ? !is(t[3], at::kByte, dev, q2) || !is(t[6], at::kByte, dev, s2) : t[3] || t[6]) ||
+            !is(t[7], at::kFloat, dev, tk) || !is_index(t[8], dev, tk))
+            Py_RETURN_NONE;
+        void* s;
+        const int here = stream_here(*x, &s);
+        if (here < 0) return nullptr;
+        if (here == 0) Py_RETURN_NONE;
+        void* p[11];
+        for (int i = 0; i < 11; ++i) p[i] = t[i] ? t[i]->data_ptr() : nullptr;
+        const uint32_t code = (uint32_t)dtype_code(ty);
+        return call([&] {
+            return g_mxfp4(p[0], p[10], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], (int)T, (int)H, (int)I,
+                           (int)E, (int)k, (int)v[2], (uint32_t)v[3], code, acc, s);
+        });
+    });
+}
+
 #define CM_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CM_METHOD(bind), CM_METHOD(topk),   CM_METHOD(forward),          CM_METHOD(router),
-                         CM_METHOD(fp8),  CM_METHOD(packed), {nullptr, nullptr, 0, nullptr}};
+                         CM_METHOD(fp8),  CM_METHOD(packed), CM_METHOD(bind_ops),         CM_METHOD(route),
+                         CM_METHOD(norm), CM_METHOD(mxfp4),  {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

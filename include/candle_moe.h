@@ -334,6 +334,78 @@ int candle_moe_fused_moe_fp8(const void* input, const void* gate_q, const void* 
                              int hidden_dim, int intermediate_dim, int num_experts, int num_selected_experts,
                              int activation_type, uint32_t moe_type, uint32_t dtype, void* stream);
 
+/* Routing with groups (no counterpart in the reference, whose router is
+ * softmax and top-k, /root/reference/src/lib.rs:124-155), for models that score
+ * experts by softmax or sigmoid, balance them by a bias and choose groups first:
+ *   s = softmax(logits[t]) (score 0) or 1 / (1 + exp(-logits[t])) (score 1);
+ *   c = s + bias (bias f32 [num_experts], or NULL: c = s);
+ *   the experts form num_groups (at most 64) groups of neighbours; a group's
+ *   score is the sum of its group_top (1 or 2) largest c; the topk_groups best
+ *   groups, then the topk largest c in them are chosen, ties to the lower index;
+ *   topk_weight = s at the chosen (descending c), divided by their sum where
+ *   renormalize is set, times scale. The bias is in the choice alone.
+ * Scores and choice in 64 bits, weights rounded to f32 once. A NaN counts as
+ * -infinity in the choice and stays a NaN in its weight; a logit of -infinity has
+ * score 0, and where all chosen have score 0 the weights are 0 (not 0 / 0).
+ *   logits [num_tokens, num_experts] of logits_dtype, 1 <= num_experts <= 1024;
+ *   topk_weight f32, topk_indices u32, token_expert_indices u32 = j * num_tokens +
+ *   t, [num_tokens, topk] each, as topk_softmax's; topk at most the
+ *   topk_groups * num_experts / num_groups experts of the chosen groups. */
+int candle_moe_topk_route(const void* logits, uint32_t logits_dtype, const float* bias, float* topk_weight,
+                          void* topk_indices, void* token_expert_indices, int num_experts, int num_tokens, int topk,
+                          int score, int num_groups, int topk_groups, int group_top, int renormalize, float scale,
+                          void* stream);
+
+/* The residual's addition and the root-mean-square norm that come before a MoE
+ * layer (no counterpart in the reference: its callers use candle's), with the
+ * 8-bit rows candle_moe_fused_moe_mxfp4 takes:
+ *   z = input + residual (input where residual is NULL), residual_output = dtype(z);
+ *   y = z / sqrt(mean(z^2) + eps) * weight, of z in f32; output = dtype(y);
+ *   codes, scales: y as MXFP8 (OCP): per 32 values along the row the byte e + 127
+ *   of the least e with max|y| <= 448 * 2^e (0 for zeros, 255 where one is not
+ *   finite), and the e4m3 code of y / 2^e, ties to even.
+ * input, residual, residual_output, output [num_tokens, hidden_dim] and weight
+ * [hidden_dim] of dtype; codes u8 [num_tokens, hidden_dim], scales u8 [num_tokens,
+ * hidden_dim / 32]. residual, residual_output, output may be NULL, codes and scales
+ * both; output or codes must be given. residual_output may be residual, and
+ * output or residual_output may be input; no other overlap. The 8-bit form needs
+ * hidden_dim a multiple of 32, at most 32768, and 16-byte aligned tensors. */
+int candle_moe_add_rms_norm(const void* input, const void* residual, const void* weight, void* residual_output,
+                            void* output, void* codes, void* scales, int num_tokens, int hidden_dim, float eps,
+                            uint32_t dtype, void* stream);
+
+/* Opt-in 4-bit expert weights (no counterpart in the reference): OCP MXFP4. A
+ * weight is an e2m1 value (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) times
+ * 2^(s - 127), s one byte for 32 weights in a row along K (255: NaN):
+ *   codes [E][N][K/2] u8, K-contiguous, even k in the low 4 bits;
+ *   scales [E][N][K/32] u8.
+ * quantize_mxfp4: weights [E][K][N] (input_kn = 1) or [E][N][K] (input_kn = 0) in
+ * dtype 0/1/2, k_dim a multiple of 32; s the least with max|w| <= 6 * 2^(s - 127)
+ * (0 for zeros, 255 with zero codes where a weight is not finite), codes to the
+ * nearest value, ties to the even code. */
+int candle_moe_quantize_mxfp4(const void* weights, uint32_t dtype, int num_experts, int k_dim, int n_dim, int input_kn,
+                              void* codes, void* scales, void* stream);
+/* out [E][N][K] of dtype = dtype(value * 2^(s - 127)), the weights the MoE below
+ * multiplies by: exact in f32 and bf16, in f16 rounded outside its range. */
+int candle_moe_dequantize_mxfp4(const void* codes, const void* scales, int num_experts, int n_dim, int k_dim, void* out,
+                                uint32_t dtype, void* stream);
+/* MoE over 4-bit weights, shapes as candle_moe_fused_moe_fp8's: Qwen3 (moe_type
+ * 0) gate_q / up_q codes of [E][I][H], down_q of [E][H][I]; Nomic (moe_type 1)
+ * gate_q = fc1 [E][I][H], up_q = fc2 [E][H][I], down_q and down_scale unused.
+ * input [num_tokens, hidden_dim] of dtype (f16, bf16) with input_scale NULL, or
+ * the MXFP8 codes of candle_moe_add_rms_norm with their scales [num_tokens,
+ * hidden_dim / 32] in input_scale, counted as dtype(value) (exact in bf16).
+ * f32 accumulation; the intermediate is rounded to dtype. accumulate != 0:
+ * output += result, else output = result. hidden_dim and intermediate_dim
+ * multiples of 32; input, codes and output 16-byte aligned. The workspace is
+ * the library's, as fused_moe's (one call of the largest size before capturing
+ * serves every smaller one). */
+int candle_moe_fused_moe_mxfp4(const void* input, const void* input_scale, const void* gate_q, const void* up_q,
+                               const void* down_q, const void* gate_scale, const void* up_scale, const void* down_scale,
+                               const void* routing_weights, const void* expert_indices, void* output, int num_tokens,
+                               int hidden_dim, int intermediate_dim, int num_experts, int num_selected_experts,
+                               int activation_type, uint32_t moe_type, uint32_t dtype, int accumulate, void* stream);
+
 /* Releases the library-owned workspaces of fused_moe / candle_moe_fused_moe_status,
  * the FusedMoE forward and candle_moe_router_topk (hipFree: waits for the
  * device, so the streams they were used on may already be destroyed; not
