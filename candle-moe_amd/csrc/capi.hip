@@ -157,7 +157,7 @@ struct Problem {
 
 // CUs per XCD of the current device (its CUs over the 8 XCDs of MI355X), 0
 // when unknown; read once per device.
-static int cus_per_xcd() {
+int cus_per_xcd() {
     static std::mutex mu;
     static int cached[64];
     static bool known[64] = {};
@@ -379,7 +379,7 @@ static size_t dec_part_bytes(const Problem& p) {
     return std::max(std::max(n1, n2) * 4, p.dtype == kF32 ? (size_t)kDecPartBytesF32 : 0);
 }
 // Workgroups of one round of the decode kernels: two per CU.
-static int dec_cap() { return 2 * 8 * std::max(cus_per_xcd(), 32); }
+int dec_cap() { return 2 * 8 * std::max(cus_per_xcd(), 32); }
 // Most pairs the decode kernels take by default (16-bit weights; up to 32
 // per touched expert). Beyond, their items outnumber one round of
 // workgroups and the 32-row kernel is faster: Qwen3-30B-A3B steps at T=32 /
@@ -778,7 +778,7 @@ struct Fp8Weights {
 // or 2 (blocks of 48 and 96 columns put Qwen3's 1536 and Nomic's 3072
 // columns of 8 experts into 256 items).
 // f32: 4 columns (the same 16 bytes per lane and k-row; slices even out the items).
-static int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32) {
+int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32, int most) {
     if (f32) return 4;
     if (ks_lim > 1) return 8;
     const double cus = 8.0 * std::max(cus_per_xcd(), 32);
@@ -788,6 +788,7 @@ static int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32) {
     int best = cand[0];
     double best_b = -1.0;
     for (int i = 0; i < ncand; ++i) {
+        if (cand[i] > most) continue;
         const double items = (double)groups * cdiv(N, 16 * cand[i]);
         const double b = items / std::ceil(items / cus);
         if (b > best_b + 1e-9) {

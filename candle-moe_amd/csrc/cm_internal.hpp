@@ -343,6 +343,10 @@ struct DecArgs {
     int w8;                   // fp8 e4m3 codes [E][N][K] (ldb = K) with f32 scales [E][N]
     const float* scale0;      // (w8) gate / fc1 column scales (kGateUp / kFc1 with ks == 1)
     const float* scale1;      // (w8) up column scales
+    int w4;                   // MXFP4 codes [E][N][K/2] (ldb = K), K a multiple of 32
+    const uint8_t* mx0;       // (w4) scale bytes [E][N][K/32] of B0
+    const uint8_t* mx1;       // (w4) and of B1
+    const uint8_t* xs;        // (w4, kGateUp / kFc1) A is MXFP8 codes: their scale bytes [T][K/32]
 };
 hipError_t launch_dec_gemv(int mode, int dtype, const DecArgs& a, hipStream_t stream);
 // Finishing the K slices of a decode GEMM (fixed slice order: deterministic),
@@ -401,6 +405,10 @@ hipError_t launch_finalize(void* out, int dtype, const float* acc, long long n, 
 int set_error(int code, const char* fmt, ...);
 void clear_error();
 int hip_fail(hipError_t e, const char* what);
+int cus_per_xcd();  // CUs of the current device over its 8 XCDs, 0 if unknown
+// Decode GEMMs: workgroups of one round; columns per lane (capi.hip)
+int dec_cap();
+int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32, int most = 8);
 // The library-owned workspace of (current device, s), held until `lock` goes.
 // need: bytes a call takes; reserve (>= need): bytes to have for the calls to come.
 struct WsLease {

@@ -147,6 +147,45 @@ __device__ __forceinline__ u32x4 fp8x8_to(const u32x2& v) {
     return r;
 }
 
+// Eight MXFP4 weights (e2m1 codes, lowest half-byte first) or MXFP8 values (e4m3
+// bytes) times their scale as the MFMA operand of the activation dtype: the
+// gfx950 scaled conversions take the power of two as an f32 of that exponent
+// byte, 0 as 2^-127 and 255 as NaN, and round to nearest even where the dtype
+// does not hold the product (f16 only), as dequantize_mxfp4 does (checked for
+// every scale and code).
+template <int DT>
+__device__ __forceinline__ u32x4 mx4x8_to(uint32_t v, float scale) {
+    u32x4 r;
+    if constexpr (DT == kBF16) {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, scale, 0));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, scale, 1));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, scale, 2));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, scale, 3));
+    } else {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, scale, 0));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, scale, 1));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, scale, 2));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v, scale, 3));
+    }
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ u32x4 mx8x8_to(const u32x2& v, float scale) {
+    u32x4 r;
+    if constexpr (DT == kBF16) {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[0], scale, false));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[0], scale, true));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[1], scale, false));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[1], scale, true));
+    } else {
+        r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[0], scale, false));
+        r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[0], scale, true));
+        r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[1], scale, false));
+        r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[1], scale, true));
+    }
+    return r;
+}
+
 // Split-K fixup. Every split writes its f32 partial tile to partial slot
 // slot0 + ks (per wave, per 32x32 block, 4 registers of a lane as one 16-byte
 // chunk, lanes contiguous), then counts itself in a.counters[ctr]; the split

@@ -61,14 +61,21 @@ __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f3
     }
 }
 
+// Weight formats of moe_dec_gemv beside the activation dtype
+enum DecWeights : int { kDecFp8 = 1, kDecMxfp4 = 2 };
+
 constexpr int kDvWaves = 4;  // waves per workgroup
 constexpr int kDvStep = 32;  // K per step (one MFMA deep)
 // steps in flight per wave: 4, or 2 for 6 or 8 columns per lane, so that a
 // wave stays within 256 registers and two workgroups share a CU; halved where
 // each column takes WCH = 2 chunks of 16 bytes per step (the same bytes in
-// flight). f32 (4 columns): twice the bytes per weight, so 2 steps.
-template <int CPL, int WCH = 1, bool F32 = false>
-constexpr int dec_ring() { return F32 ? 2 : (CPL >= 6 ? 2 : 4) / WCH; }
+// flight). f32 (4 columns): twice the bytes per weight, so 2 steps. MXFP4: a step
+// is 128 k, whose rows take four loads each, so fewer with two row blocks.
+template <int CPL, int WCH = 1, bool F32 = false, bool W4 = false, int RB = 1>
+constexpr int dec_ring() {
+    if (W4) return CPL >= 6 || (RB == 2 && CPL > 2) ? 2 : CPL == 4 ? 3 : 4;
+    return F32 ? 2 : (CPL >= 6 ? 2 : 4) / WCH;
+}
 
 // Operand j of a transposed 8 x CPL block: r[t] holds k-row t of CPL
 // consecutive columns (pairs of 16-bit values, low half first); the result
@@ -286,13 +293,14 @@ __device__ __forceinline__ void finish_token4(const DecFinish& f, int ks, long l
     }
 }
 
-template <int DT, int MODE, int RB, int CPL, bool PK, bool W8>
+template <int DT, int MODE, int RB, int CPL, bool PK, int WQ, bool X8 = false>
 __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     constexpr bool DUAL = (MODE == kGateUp);
     constexpr bool GATHER = (MODE == kGateUp || MODE == kFc1);
     // [K,N] weights (the API layout but Nomic's fc2); [N,K]: fc2, every GEMM
-    // on pre-packed weights (PK) and on fp8 codes (W8)
-    constexpr bool TRANS = (MODE != kFc2Rows) && !PK && !W8;
+    // on pre-packed weights (PK) and on fp8 (W8) or MXFP4 (W4) codes
+    constexpr bool W8 = WQ == kDecFp8, W4 = WQ == kDecMxfp4;
+    constexpr bool TRANS = (MODE != kFc2Rows) && !PK && !W8 && !W4;
     // W8: OCP fp8 e4m3 codes [E][N][K] (one byte per weight) with per-column
     // f32 scales. A step is 128 k: a lane's two 16-byte loads hold
     // k0 + 32g .. +31 of its column, the operands of four MFMAs (converted
@@ -311,14 +319,20 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     // form (whose v_perm transpose the pairwise conversion replaces); [N,K]:
     // two 16-byte chunks of 4 k, 128 contiguous bytes per column and step.
     constexpr bool F32 = DT == kF32;
-    static_assert(!F32 || (!W8 && !PK && CPL == 4), "f32: API layout, 4 columns per lane");
-    constexpr int WCH = (W8 || MODE == kFc2Rows) ? 2 : 1;
-    constexpr int KSTEP = F32 ? kDvStep : (W8 ? 64 : kDvStep) * WCH;
-    constexpr int KG = F32 ? 8 : (W8 ? 16 : 8) * WCH;  // k per lane group per step
-    constexpr int KC = F32 ? 8 / WCH : W8 ? 16 : 8;    // k per weight chunk
-    constexpr int WB = F32 ? 4 : W8 ? 1 : 2;           // bytes per weight
-    constexpr int AB = F32 ? 4 : 2;                    // bytes per activation
-    constexpr int AH = F32 ? 2 : (W8 ? 2 : 1) * WCH;   // 16-byte A loads per row and step
+    static_assert(!F32 || (!W8 && !W4 && !PK && CPL == 4), "f32: API layout, 4 columns per lane");
+    // W4: MXFP4 codes [E][N][K/2]; a lane's 16-byte chunk holds the 32 k of one
+    // scale (scales [E][N][K/32], a byte load beside it), which the gfx950 scaled
+    // conversion applies while it turns the codes into DT operands, exactly.
+    // X8: the rows are MXFP8 codes with a scale byte per 32 k (xs), converted the
+    // same way.
+    static_assert(!X8 || (W4 && GATHER), "8-bit rows: gate/up and fc1 over MXFP4 weights");
+    constexpr int WCH = (W8 || (MODE == kFc2Rows && !W4)) ? 2 : 1;
+    constexpr int KSTEP = F32 ? kDvStep : (W4 ? 128 : W8 ? 64 : kDvStep) * WCH;
+    constexpr int KG = F32 ? 8 : (W4 ? 32 : W8 ? 16 : 8) * WCH;  // k per lane group per step
+    constexpr int KC = F32 ? 8 / WCH : W4 ? 32 : W8 ? 16 : 8;    // k per weight chunk
+    constexpr int WBITS = F32 ? 32 : W4 ? 4 : W8 ? 8 : 16;       // bits per weight
+    constexpr int AB = F32 ? 4 : X8 ? 1 : 2;                     // bytes per activation
+    constexpr int AH = F32 ? 2 : KG * AB / 16;                   // 16-byte A loads per row and step
     constexpr bool ROWS = (MODE == kDownRows || MODE == kFc2Rows);
     constexpr int NT = 64 * kDvWaves;
     constexpr int WGC = 16 * CPL;                // output columns per workgroup
@@ -360,9 +374,17 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     const int col0 = cb * WGC;
 
     // weights of expert e (this wave's tensor): in-range loads only, zeros past
-    const char* wbase = reinterpret_cast<const char*>(tensor ? a.B1 : a.B0) + (long long)e * a.strideB * WB;
+    const long long wbytes = a.strideB * WBITS / 8;
+    const char* wbase = reinterpret_cast<const char*>(tensor ? a.B1 : a.B0) + (long long)e * wbytes;
     const __amdgpu_buffer_rsrc_t rw =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(wbase), 0, (int)(a.strideB * WB), 0x00020000);
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(wbase), 0, (int)wbytes, 0x00020000);
+    // (W4) the expert's scale bytes; (X8) the rows'
+    const long long sbytes = a.strideB / 32;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        W4 ? const_cast<uint8_t*>(tensor ? a.mx1 : a.mx0) + (long long)e * sbytes : nullptr, 0, W4 ? (int)sbytes : 0,
+        0x00020000);
+    const __amdgpu_buffer_rsrc_t rxs = __builtin_amdgcn_make_buffer_rsrc(
+        X8 ? const_cast<uint8_t*>(a.xs) : nullptr, 0, X8 ? (int)(a.a_bytes / 32) : 0, 0x00020000);
     const __amdgpu_buffer_rsrc_t rx =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.A), 0, (int)a.a_bytes, 0x00020000);
 
@@ -370,7 +392,7 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     // whole number of ring rounds (the steps past s_hi load zeros), so that
     // the ring loop needs no guard. The parts depend on K, the slices and the
     // waves only (not on the ring or the column block).
-    constexpr int RING = dec_ring<CPL, WCH, F32>();
+    constexpr int RING = dec_ring<CPL, WCH, F32, W4, RB>();
     const int nks = (K + KSTEP - 1) / KSTEP;
     const int nparts = KP * ks;
     const int per = (nks + nparts - 1) / nparts;
@@ -388,21 +410,23 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     // [N,K]: column ncol[b], k KG*g. A lane whose columns lie past N starts at
     // kOob. (Every offset stays below 2^32: kOob plus less than the expert's
     // 2^31 bytes.)
-    const uint32_t ldb2 = (uint32_t)a.ldb * (uint32_t)WB;  // bytes per weight row
+    const uint32_t ldb2 = (uint32_t)a.ldb * (uint32_t)WBITS / 8u;  // bytes per weight row
     uint32_t wlane[TRANS ? 1 : NB];
 #pragma unroll
     for (int b = 0; b < (TRANS ? 1 : NB); ++b)
-        wlane[b] = ncol[b] < N ? (TRANS ? 8u * (uint32_t)g * ldb2 + (uint32_t)WB * (uint32_t)ncol[0]
-                                        : (uint32_t)ncol[b] * ldb2 + (uint32_t)(KG * WB) * (uint32_t)g)
+        wlane[b] = ncol[b] < N ? (TRANS ? 8u * (uint32_t)g * ldb2 + (uint32_t)(WBITS / 8) * (uint32_t)ncol[0]
+                                        : (uint32_t)ncol[b] * ldb2 + (uint32_t)(KG * WBITS / 8) * (uint32_t)g)
                                : kOob;
 
     // ring of steps: weight chunks (CPL 16-bit values each for [K,N], 8 for
     // [N,K]) and the A rows. Branch-free offsets (a branch, or a select on
     // the step alone, made the compiler wait for every load in flight): a
     // lane's k positions past K read zeros (kOob).
-    constexpr int WDW = TRANS ? CPL * WB / 4 : 4;  // dwords per weight load
+    constexpr int WDW = TRANS ? CPL * WBITS / 32 : 4;  // dwords per weight load
     uint32_t wv[RING][NLD][WDW];
     u32x4 xv[RING][RB][AH];
+    uint32_t sv[W4 ? RING : 1][W4 ? NLD : 1];         // scale bytes of the chunks
+    uint32_t xsv[X8 ? RING : 1][RB][X8 ? WCH : 1];    // and of the rows' 32 k
     // this lane's k of step s, chunk c, inside the wave's part and K (K is a
     // multiple of KC: a chunk lies wholly inside or outside). Bitwise, not
     // short-circuit: a branch on the uniform s < s_hi made the compiler wait
@@ -418,7 +442,9 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
             const bool kok = k_ok(s, c);
             uint32_t o;
             if constexpr (TRANS) o = kok ? wlane[0] + (uint32_t)(s * KSTEP + t) * ldb2 : kOob;
-            else o = kok ? wlane[t / WCH] + (uint32_t)(s * KSTEP * WB + 16 * c) : kOob;
+            else o = kok ? wlane[t / WCH] + (uint32_t)(s * (KSTEP * WBITS / 8) + 16 * c) : kOob;
+            if constexpr (W4)
+                sv[i][t] = __builtin_amdgcn_raw_buffer_load_b8(rs, kok ? o / 16u : kOob, 0, 0);
             if constexpr (WDW == 4) {
                 const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rw, o, 0, 0);
 #pragma unroll
@@ -448,7 +474,7 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     for (int c0 = 0; c0 < cnt; c0 += RB * 16) {
         const int m_valid = min(RB * 16, cnt - c0);
         // A rows of this lane (row li of each row block), k 8g
-        uint32_t abase[RB];
+        uint32_t abase[RB];  // (X8: a scale byte is at abase / 32)
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             const int m = rb * 16 + li;
@@ -479,6 +505,11 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
                     const bool kok = k_ok(s, h / (AH / WCH));
                     xv[i][rb][h] = __builtin_amdgcn_raw_buffer_load_b128(
                         rx, kok ? abase[rb] + (uint32_t)(s * KSTEP * AB) + 16u * h : kOob, 0, 0);
+                    if constexpr (X8) {
+                        if (h % 2 == 0)
+                            xsv[i][rb][h / 2] = __builtin_amdgcn_raw_buffer_load_b8(
+                                rxs, kok ? (abase[rb] + (uint32_t)(s * KSTEP)) / 32u + (uint32_t)(h / 2) : kOob, 0, 0);
+                    }
                 }
         };
         auto load = [&](int i, int st) {
@@ -496,6 +527,37 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
                                         __uint_as_float(y[2]), __uint_as_float(y[3])};
                     split8(v, ap[rb][0], ap[rb][1], ap[rb][2]);
                 }
+            }
+            if constexpr (W4) {
+                // chunk c: 32 k of column b and of the row, as four operands of 8 k
+#pragma unroll
+                for (int c = 0; c < WCH; ++c) {
+                    u32x4 ao[RB][4];
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            if constexpr (X8) {
+                                const u32x4& x = xv[i][rb][2 * c + m / 2];
+                                ao[rb][m] = mx8x8_to<DT>(u32x2{x[2 * (m & 1)], x[2 * (m & 1) + 1]},
+                                                         __uint_as_float(xsv[i][rb][c] << 23));
+                            } else {
+                                ao[rb][m] = xv[i][rb][4 * c + m];
+                            }
+                        }
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        const uint32_t(&w)[WDW] = wv[i][b * WCH + c];
+                        const float sc = __uint_as_float(sv[i][b * WCH + c] << 23);
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            const u32x4 wo = mx4x8_to<DT>(w[m], sc);
+#pragma unroll
+                            for (int rb = 0; rb < RB; ++rb) acc[rb][b] = mfma16<DT>(ao[rb][m], wo, acc[rb][b]);
+                        }
+                    }
+                }
+                return;
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -782,26 +844,40 @@ hipError_t launch_cfg(const DecArgs& a, hipStream_t stream) {
     if (a.max_groups <= 0) return hipSuccess;
     const dim3 grid((int)nwg), block(64 * kDvWaves);
     if constexpr (DT != kF32) {
+        // fp8 and MXFP4 codes are [N,K] for every GEMM (Nomic's fc2 runs the down mode)
+        constexpr int M8 = MODE == kFc2Rows ? kDownRows : MODE;
         if (a.w8) {
-            // fp8 codes are [N,K] for every GEMM (Nomic's fc2 runs the down mode)
-            constexpr int M8 = MODE == kFc2Rows ? kDownRows : MODE;
-            hipLaunchKernelGGL((moe_dec_gemv<DT, M8, RB, CPL, false, true>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((moe_dec_gemv<DT, M8, RB, CPL, false, kDecFp8>), grid, block, 0, stream, a);
             return hipGetLastError();
+        }
+        if (a.w4) {
+            // (two row blocks of 8 columns per lane would not fit 256 registers)
+            if constexpr (RB == 2 && CPL == 8) return hipErrorInvalidValue;
+            else {
+            if constexpr (M8 != kDownRows) {
+                if (a.xs) {
+                    hipLaunchKernelGGL((moe_dec_gemv<DT, M8, RB, CPL, false, kDecMxfp4, true>), grid, block, 0, stream, a);
+                    return hipGetLastError();
+                }
+            }
+            hipLaunchKernelGGL((moe_dec_gemv<DT, M8, RB, CPL, false, kDecMxfp4>), grid, block, 0, stream, a);
+            return hipGetLastError();
+            }
         }
     }
     if constexpr (DT == kF32) {
-        hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, false, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, false, 0>), grid, block, 0, stream, a);
         return hipGetLastError();
     }
     // (Nomic's fc2 is [N,K] either way: no packed instance)
     if constexpr (MODE != kFc2Rows && DT != kF32) {
         if (a.packed) {
-            hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, true, false>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, true, 0>), grid, block, 0, stream, a);
             return hipGetLastError();
         }
     }
     if constexpr (DT != kF32 && (MODE == kFc2Rows || (CPL != 3 && CPL != 6))) {
-        hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, false, false>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, false, 0>), grid, block, 0, stream, a);
         return hipGetLastError();
     }
     return hipErrorInvalidValue;  // [K,N] weights: 2, 4 or 8 columns per lane
