@@ -134,6 +134,8 @@ struct Problem {
     bool f32_tiled;  // f32 operands the split-bf16 kernels can load (16-byte chunks of 4 k)
     bool f32_dec;    // and the decode kernels (8 k)
     bool fp8;
+    bool mx;      // MXFP4 weights (candle_moe_fused_moe_mxfp4): f32 pair rows
+    bool mx8;     // and MXFP8 rows, expanded to 16 bits but by the decode kernels
     bool packed;  // pre-packed K-contiguous 16-bit weights (candle_moe_fused_moe_packed)
     int cfg;  // TileCfg of both GEMMs
     int BM;
@@ -157,7 +159,7 @@ struct Problem {
 
 // CUs per XCD of the current device (its CUs over the 8 XCDs of MI355X), 0
 // when unknown; read once per device.
-int cus_per_xcd() {
+static int cus_per_xcd() {
     static std::mutex mu;
     static int cached[64];
     static bool known[64] = {};
@@ -182,7 +184,7 @@ struct Layout {
     size_t sync;  // 4 ints of the one-launch grouping (offset 0, 256 bytes)
     size_t offsets, block_counts, sorted_pair, tile_row, tile_exp, num_tiles;
     size_t k_offsets, k_block_counts, tok_sorted, tile_row2, tile_key2, num_tiles2, pair_dest;
-    size_t inter, acc, partial, counters, dec_meta, total;
+    size_t inter, acc, partial, counters, dec_meta, rows16, total;
 };
 
 // 0: choose per call; 1: always the pair path (pair rows or f32 atomics,
@@ -278,8 +280,10 @@ static Layout make_layout(const Problem& p) {
     if (p.cfg == kDecGemv) {
         o += a256(dec_part_bytes(p));  // decode kernels
     } else if (!p.set_path) {
-        o += p.rows_path ? a256((size_t)p.P * p.H * es) : a256((size_t)p.T * p.H * 4);
+        o += p.rows_path ? a256((size_t)p.P * p.H * (p.mx ? 4 : es)) : a256((size_t)p.T * p.H * 4);
     }
+    L.rows16 = o;  // MXFP8 rows in 16 bits
+    if (p.mx8 && p.cfg != kDecGemv) o += a256((size_t)p.T * p.H * 2);
     // split-K partials and arrival counters, shared by the two GEMMs (they run
     // one after the other; the counters are left zero)
     L.dec_meta = o;
@@ -365,6 +369,7 @@ static void choose_dec_slices(Problem& p) {
     // 34.3), H 8192 I 2048 k 1 T=1 85.6 / 37.9, H 4096 I 512 E 128 k 8 T=1
     // 51.0 / 32.2. At 96 blocks (Qwen3 T=2) 57.9 / 43.0, but pre-packed,
     // which takes the same slices to give the same bits, 48.2 / 51.1.
+    if (p.mx) return;  // (as fp8: half its bytes)
     const bool few = !p.fp8 && groups * cdiv(p.I, 64) <= 64 &&
                      (long long)(q3 ? 2 : 1) * p.H * 64 * (p.dtype == kF32 ? 4 : 2) >= (p.dtype == kF32 ? 1 << 19 : 1 << 20);
     if (groups * cdiv(p.I, cols) < 256 && (wbytes >= kDecSliceBytes || few))
@@ -379,7 +384,7 @@ static size_t dec_part_bytes(const Problem& p) {
     return std::max(std::max(n1, n2) * 4, p.dtype == kF32 ? (size_t)kDecPartBytesF32 : 0);
 }
 // Workgroups of one round of the decode kernels: two per CU.
-int dec_cap() { return 2 * 8 * std::max(cus_per_xcd(), 32); }
+static int dec_cap() { return 2 * 8 * std::max(cus_per_xcd(), 32); }
 // Most pairs the decode kernels take by default (16-bit weights; up to 32
 // per touched expert). Beyond, their items outnumber one round of
 // workgroups and the 32-row kernel is faster: Qwen3-30B-A3B steps at T=32 /
@@ -387,6 +392,8 @@ int dec_cap() { return 2 * 8 * std::max(cus_per_xcd(), 32); }
 // the decode kernels against 115 / 126 / 134 / 149 us; Qwen3 T=128 (256
 // pairs) 102 against 115 us.
 constexpr long long kDecDefaultPairs = 256;
+// MXFP4 weights: the same
+constexpr long long kMxDecPairs = 256;
 // 16-bit prefill batches: rows per touched expert up to which nearly every
 // expert's rows fit one extended 128-row tile (160 rows: two standard
 // deviations of uniform routing above), and from which a 256-row tile often
@@ -404,7 +411,7 @@ constexpr long long kTwoTileRows = 232;
 // f32_dec: f32 calls may take the decode kernels.
 static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t moe_type, uint32_t dtype,
                          Problem& p, bool aligned16 = true, bool out16 = true, bool fp8 = false,
-                         bool packed = false, bool f32_dec = true) {
+                         bool packed = false, bool f32_dec = true, bool mx = false, bool mx8 = false) {
     if (T < 0) return set_error(CANDLE_MOE_ERR_INVALID, "fused_moe: num_tokens must be >= 0 (got %d)", T);
     if (H < 1 || I < 1)
         return set_error(CANDLE_MOE_ERR_INVALID, "fused_moe: hidden_dim and intermediate_dim must be >= 1 (got %d, %d)", H, I);
@@ -421,6 +428,8 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
     p.P = P;
     p.mfma = mfma_supported(p.dtype, H, I) && mfma_supported(p.dtype, I, H) && aligned16;
     p.packed = packed;
+    p.mx = mx;
+    p.mx8 = mx8;
     if (packed && !p.mfma)
         return set_error(CANDLE_MOE_ERR_UNSUPPORTED,
                          "fused_moe_packed: needs f16 or bf16, hidden_dim and intermediate_dim multiples of 8 and "
@@ -497,6 +506,15 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
         if (g_tile_policy == kW8Gemv || g_tile_policy == kLdsRows32 || g_tile_policy == kLds256w8 ||
             (g_tile_policy == kDecGemv && dec_gemv_fits(p)))
             p.cfg = g_tile_policy;
+    } else if (mx) {
+        if (!p.mfma || H % 32 || I % 32)
+            return set_error(CANDLE_MOE_ERR_UNSUPPORTED,
+                             "fused_moe_mxfp4: needs f16 or bf16, hidden_dim and intermediate_dim multiples of 32 and "
+                             "16-byte aligned tensors (got dtype %u, %d, %d)", dtype, H, I);
+        p.cfg = P <= 32 * touched ? kLdsRows32 : P <= kOneTileRows * touched ? kLds128 : kLds256w8;
+        if (P <= kMxDecPairs && dec_gemv_fits(p)) p.cfg = kDecGemv;
+        if ((is_lds_cfg(g_tile_policy) && g_tile_policy != kW8Gemv) || (g_tile_policy == kDecGemv && dec_gemv_fits(p)))
+            p.cfg = g_tile_policy;
     } else if (p.mfma && !policy) {
         const long long dev_wgs = 8LL * std::max(cus_per_xcd(), 32);
         const long long wgs256 = est_tiles(256) * cdiv(I, gemm_tile_cols(p.moe_type == kQwen3 ? kGateUp : kFc1, kLds256w8));
@@ -548,6 +566,7 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
         const long long lim = 0x7fffff00LL;
         if ((long long)T * H * es >= lim || P * I * es >= lim || (long long)H * I * es >= lim) {
             if (fp8) return set_error(CANDLE_MOE_ERR_UNSUPPORTED, "fused_moe_fp8: operands beyond 2 GiB");
+            if (mx) return set_error(CANDLE_MOE_ERR_UNSUPPORTED, "fused_moe_mxfp4: operands beyond 2 GiB");
             p.cfg = kTile128;
         }
     }
@@ -585,7 +604,7 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
             const bool big_rows = (double)P * H * 2.0 >= (double)kSetMinRowBytes;
             p.set_from = std::max(fill * 256 * sets, kSetMinRowBytes / (2.0 * H * k));
             p.set_path = p.cfg != kDecGemv &&
-                         (g_combine_policy == 2 ||
+                         ((g_combine_policy == 2 && !(mx && p.cfg == kLdsRows32)) ||
                           (p.cfg != kLdsRows32 && (double)T >= fill * p.BM * sets && (!rows_ok || big_rows)));
         }
     }
@@ -613,7 +632,8 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
     // (Qwen3-30B-A3B T=16: 90 against 94 us).
     p.rows_path = p.cfg == kDecGemv ||
                   (!p.set_path && p.lds_family && p.dtype != kF32 && p.cfg != kLdsRows32 && p.cfg != kW8Gemv &&
-                   (double)P * H * 2.0 <= kRowsMaxBytes);
+                   (double)P * H * 2.0 <= kRowsMaxBytes) ||
+                  (!p.set_path && mx);
     // extended row tiles on the 16-bit LDS-DMA kernels that have them (not with
     // the f32-atomic combine, whose kernels share the tile table)
     p.ext = (p.set_path || p.rows_path) && !fp8 ? ext_rows_of(p.cfg) : 0;
@@ -706,8 +726,8 @@ static size_t upto_bytes(const Problem& p) {
 
     size_t acc = 0, partial = 0;
     // decode kernels: the partials of both GEMMs by slices
-    const bool any_rows = p.fp8 || g_tile_policy == kDecGemv;  // (else up to 32 rows per touched expert)
-    const long long most = g_tile_policy == kDecGemv ? kDecMaxPairs : p.fp8 ? kW8DecPairs : kDecDefaultPairs;
+    const bool any_rows = p.fp8 || p.mx || g_tile_policy == kDecGemv;  // (else up to 32 rows per touched expert)
+    const long long most = g_tile_policy == kDecGemv ? kDecMaxPairs : p.fp8 ? kW8DecPairs : p.mx ? kMxDecPairs : kDecDefaultPairs;
     const long long dec_pairs = any_rows ? most : std::min(most, 32 * E);
     Problem q = p;
     q.cfg = kDecGemv;
@@ -734,6 +754,13 @@ static size_t upto_bytes(const Problem& p) {
             partial = splits(32, forced ? P : std::min(P, 64 * E));
             if (forced || P > 64 * touched) partial = std::max(partial, splits(128, P));
         } else {
+            if (p.mx) {
+                // f32 pair rows on every kernel, until the expert sets take over
+                double t = p.T;
+                if (p.set_path && g_combine_policy == 0) t = std::min(t, std::ceil(p.set_from));
+                acc = std::max(acc, (size_t)(t * p.k * p.H * 4.0));
+                if (p.mx8) o += a256((size_t)p.T * p.H * 2);
+            }
             // 32-row kernels: f32 atomics, one round of K splits
             const long long rows32 = forced ? P : std::min(P, (p.fp8 ? 256 : 128) * E);
             acc = std::max(acc, (size_t)(rows32 / p.k) * p.H * 4);
@@ -778,7 +805,7 @@ struct Fp8Weights {
 // or 2 (blocks of 48 and 96 columns put Qwen3's 1536 and Nomic's 3072
 // columns of 8 experts into 256 items).
 // f32: 4 columns (the same 16 bytes per lane and k-row; slices even out the items).
-int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32, int most) {
+static int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32, int most) {
     if (f32) return 4;
     if (ks_lim > 1) return 8;
     const double cus = 8.0 * std::max(cus_per_xcd(), 32);
@@ -800,8 +827,9 @@ int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32, int most)
 }
 static int run_moe_dec(const Problem& p, const void* x, const void* gate, const void* up, const void* down,
                        const float* rw, const uint32_t* idx, void* out, bool overwrite, char* ws, const Layout& L,
-                       hipStream_t s, const Fp8Weights* f8) {
+                       hipStream_t s, const Fp8Weights* f8, const MxWeights* mx) {
     const bool qwen3 = p.moe_type == kQwen3;
+    const bool nk = p.packed || f8 || mx;  // every weight matrix [N,K]
     void* inter = ws + L.inter;
     float* part = reinterpret_cast<float*>(ws + L.acc);
     int* meta = reinterpret_cast<int*>(ws + L.dec_meta);
@@ -820,20 +848,27 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     d.k_top = p.k;
     d.act = p.act;
     d.strideB = (long long)p.H * p.I;
-    d.ldb = (p.packed || f8) ? p.H : p.I;  // gate / up [E][H][I], or packed / fp8 codes [E][I][H]
+    d.ldb = nk ? p.H : p.I;  // gate / up [E][H][I], or packed / fp8 / MXFP4 codes [E][I][H]
     d.packed = p.packed ? 1 : 0;
     if (f8) {
         d.w8 = 1;
         d.scale0 = f8->gate_scale;
         d.scale1 = f8->up_scale;
     }
+    if (mx) {
+        d.w4 = 1;
+        d.mx0 = mx->gate_s;
+        d.mx1 = mx->up_s;
+        d.xs = mx->x_s;
+    }
     const int es = p.dtype == kF32 ? 4 : 2;
-    d.a_bytes = (long long)p.T * p.H * es;
+    d.a_bytes = (long long)p.T * p.H * (mx && mx->x_s ? 1 : es);
     d.max_groups = (int)std::min<long long>(p.P, p.E);
     d.rows_max = (int)std::min<long long>(p.P, p.T);
     d.cap = dec_cap();
     d.ks_lim = p.dec_ks1;
-    d.cpl = dec_cpl(d.max_groups, p.I, !p.packed && !f8, d.ks_lim, p.dtype == kF32);
+    const int most_cpl = mx && d.rows_max > 16 ? 6 : 8;  // (launch_cfg)
+    d.cpl = dec_cpl(d.max_groups, p.I, !nk, d.ks_lim, p.dtype == kF32, most_cpl);
     d.nblk = cdiv(p.I, 16 * d.cpl);
     const int mode1 = qwen3 ? kGateUp : kFc1;
     hipError_t e;
@@ -866,7 +901,11 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     d2.C = nullptr;
     d2.K = p.I;
     d2.N = p.H;
-    d2.ldb = (qwen3 && !p.packed && !f8) ? p.H : p.I;  // down [E][I][H] (packed / fp8 [E][H][I]); fc2 [E][H][I]
+    d2.ldb = (qwen3 && !nk) ? p.H : p.I;  // down [E][I][H] (packed / fp8 / MXFP4 [E][H][I]); fc2 [E][H][I]
+    if (mx) {
+        d2.mx0 = qwen3 ? mx->down_s : mx->up_s;
+        d2.mx1 = d2.xs = nullptr;
+    }
     d2.a_bytes = p.P * p.I * es;
     d2.ks_lim = p.dec_ks2;
     // fp8 column scales: multiplied in by the GEMM when it is not K-sliced
@@ -874,7 +913,7 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     const float* s2 = f8 ? (qwen3 ? f8->down_scale : f8->up_scale) : nullptr;
     d2.scale0 = d2.ks_lim == 1 ? s2 : nullptr;
     d2.scale1 = nullptr;
-    d2.cpl = dec_cpl(d.max_groups, p.H, qwen3 && !p.packed && !f8, d2.ks_lim, p.dtype == kF32);
+    d2.cpl = dec_cpl(d.max_groups, p.H, qwen3 && !nk, d2.ks_lim, p.dtype == kF32, most_cpl);
     d2.nblk = cdiv(p.H, 16 * d2.cpl);
     {
         ProfScope ps(kSlotGemm2, s);
@@ -908,8 +947,9 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
 // launch), which allows the one-launch grouping.
 static int run_moe(const Problem& p, const void* x, const void* gate, const void* up, const void* down,
                    const float* rw, const uint32_t* idx, void* out, bool overwrite, char* ws, hipStream_t s,
-                   const Fp8Weights* f8 = nullptr, bool sync_zero = false) {
+                   const Fp8Weights* f8 = nullptr, bool sync_zero = false, const MxWeights* mx = nullptr) {
     auto gemm = [&](int mode, const GemmArgs& g) {
+        if (mx) return launch_moe_gemm_mx(mode, p.dtype, p.cfg, g, s);
         return f8 ? launch_moe_gemm_w8(mode, p.dtype, p.cfg, g, s) : launch_moe_gemm(mode, p.dtype, p.cfg, g, s);
     };
     const Layout L = make_layout(p);
@@ -946,7 +986,14 @@ static int run_moe(const Problem& p, const void* x, const void* gate, const void
         tb.num_tiles = reinterpret_cast<int32_t*>(ws + L.num_tiles2);
         pair_dest = reinterpret_cast<int32_t*>(ws + L.pair_dest);
     }
-    if (p.cfg == kDecGemv) return run_moe_dec(p, x, gate, up, down, rw, idx, out, overwrite, ws, L, s, f8);
+    if (p.cfg == kDecGemv) return run_moe_dec(p, x, gate, up, down, rw, idx, out, overwrite, ws, L, s, f8, mx);
+    if (mx && mx->x_s) {
+        // MXFP8 rows in 16 bits, exactly (bf16): the tile kernels' operand
+        ProfScope ps(kSlotGroup, s);
+        e = launch_rows8_to(x, mx->x_s, p.T, p.H, ws + L.rows16, p.dtype, s);
+        if (e != hipSuccess) return hip_fail(e, "fused_moe_mxfp4 rows");
+        x = ws + L.rows16;
+    }
     {
         // pairs by expert and, on the expert-set path, tokens by expert set
         const GroupJob pj = pair_grouping_job(idx, p.P, p.E, p.BM, p.ext, gb);
@@ -1007,6 +1054,11 @@ static int run_moe(const Problem& p, const void* x, const void* gate, const void
         g1.scale0 = f8->gate_scale;
         g1.scale1 = f8->up_scale;
     }
+    if (mx) {  // codes [E][I][H/2]
+        g1.ldb = p.H;
+        g1.mx0 = mx->gate_s;
+        g1.mx1 = mx->up_s;
+    }
     {
         ProfScope ps(kSlotGemm1, s);
         e = gemm(mode1, g1);
@@ -1041,6 +1093,11 @@ static int run_moe(const Problem& p, const void* x, const void* gate, const void
             g2.ldb = p.I;
             g2.scale0 = qwen3 ? f8->down_scale : f8->up_scale;
             g2.scale1 = nullptr;
+        }
+        if (mx) {  // codes [E][H][I/2]
+            g2.ldb = p.I;
+            g2.mx0 = qwen3 ? mx->down_s : mx->up_s;
+            g2.mx1 = nullptr;
         }
         const int mode2 = qwen3 ? kDownSet : kFc2Set;
         g2.n_tiles = cdiv(p.H, gemm_tile_cols(mode2, p.cfg));
@@ -1083,6 +1140,11 @@ static int run_moe(const Problem& p, const void* x, const void* gate, const void
         g2.scale0 = qwen3 ? f8->down_scale : f8->up_scale;
         g2.scale1 = nullptr;
     }
+    if (mx) {  // codes [E][H][I/2]
+        g2.ldb = p.I;
+        g2.mx0 = qwen3 ? mx->down_s : mx->up_s;
+        g2.mx1 = nullptr;
+    }
     {
         ProfScope ps(kSlotGemm2, s);
         e = gemm(mode2, g2);
@@ -1091,7 +1153,9 @@ static int run_moe(const Problem& p, const void* x, const void* gate, const void
 
     {
         ProfScope ps(kSlotFinal, s);
-        e = p.rows_path ? launch_pair_rows_sum(out, p.dtype, ws + L.acc, static_cast<const uint32_t*>(idx), p.E,
+        e = mx ? launch_pair_rows32_sum(out, p.dtype, reinterpret_cast<const float*>(ws + L.acc), rw, idx, p.E, p.T, p.k,
+                                        p.H, overwrite, s)
+            : p.rows_path ? launch_pair_rows_sum(out, p.dtype, ws + L.acc, static_cast<const uint32_t*>(idx), p.E,
                                                p.T, p.k, p.H, overwrite, s)
                         : launch_finalize(out, p.dtype, acc, (long long)p.T * p.H, overwrite, s);
     }
@@ -1215,24 +1279,6 @@ static int ws_fail(const char* who, size_t need, hipError_t e) {
     return set_error(CANDLE_MOE_ERR_WORKSPACE, "%s: hipMallocAsync(%zu) failed: %s", who, need, hipGetErrorString(e));
 }
 
-int lease_workspace(const char* who, size_t need, size_t reserve, hipStream_t s, WsLease& l) {
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return hip_fail(e, who);
-    l.lock = std::unique_lock<std::mutex>(g_ws_mu);
-    OwnedWs* w = owned_ws_locked(dev, s, need, std::max(need, reserve), e);
-    if (!w) return ws_fail(who, need, e);
-    l.ptr = static_cast<char*>(w->ptr);
-    l.bytes = w->bytes;
-    return CANDLE_MOE_OK;
-}
-
-size_t packed_upto_bytes(int T, int H, int I, int E, int k, int act, uint32_t moe_type, uint32_t dtype) {
-    Problem p;
-    if (check_problem(T, H, I, E, k, act, moe_type, dtype, p, true, true, false, true)) return 0;
-    return upto_bytes(p);
-}
-
 int trim_owned_workspaces() {
     std::lock_guard<std::mutex> lk(g_ws_mu);
     int cur = 0;
@@ -1257,12 +1303,13 @@ int trim_owned_workspaces() {
 int fused_moe_impl(const void* x, const void* gate, const void* up, const void* down, const void* rw,
                    const void* idx, void* out, int T, int H, int I, int E, int k, int act, uint32_t moe_type,
                    uint32_t dtype, void* ws, size_t ws_bytes, bool own_ws, bool overwrite, void* stream,
-                   const Fp8Weights* f8, bool packed) {
+                   const Fp8Weights* f8, bool packed, const MxWeights* mx) {
     clear_error();
     Problem p;
     auto a16 = [](const void* q) { return ((uintptr_t)q & 15) == 0; };
     const bool aligned16 = a16(x) && a16(gate) && a16(up) && a16(down);
-    int rc = check_problem(T, H, I, E, k, act, moe_type, dtype, p, aligned16, a16(out), f8 != nullptr, packed);
+    int rc = check_problem(T, H, I, E, k, act, moe_type, dtype, p, aligned16, a16(out), f8 != nullptr, packed, true,
+                           mx != nullptr, mx && mx->x_s);
     if (rc) return rc;
     rc = check_ptrs(p, x, gate, up, down, rw, idx, out);
     if (rc) return rc;
@@ -1276,14 +1323,16 @@ int fused_moe_impl(const void* x, const void* gate, const void* up, const void* 
         if ((uintptr_t)ws % 256)
             return set_error(CANDLE_MOE_ERR_WORKSPACE, "fused_moe: workspace must be 256-byte aligned");
         return run_moe(p, x, gate, up, down, reinterpret_cast<const float*>(rw),
-                       reinterpret_cast<const uint32_t*>(idx), out, overwrite, reinterpret_cast<char*>(ws), s, f8);
+                       reinterpret_cast<const uint32_t*>(idx), out, overwrite, reinterpret_cast<char*>(ws), s, f8, false, mx);
     }
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
     if (e != hipSuccess) return hip_fail(e, "fused_moe: hipGetDevice");
     std::lock_guard<std::mutex> lk(g_ws_mu);
     OwnedWs* w = find_ws_locked(dev, s);
-    const long long layer[8] = {p.H, p.I, p.E, p.k, p.dtype | p.moe_type << 4 | (int)p.fp8 << 5 | (int)p.packed << 6,
+    const long long layer[8] = {p.H, p.I, p.E, p.k,
+                                p.dtype | p.moe_type << 4 | (int)p.fp8 << 5 | (int)p.packed << 6 | (int)p.mx << 7 |
+                                    (int)p.mx8 << 8,
                                 (int)aligned16 | (int)p.set_path << 1, g_tile_policy, g_combine_policy};
     int slot = -1;
     if (w)
@@ -1300,7 +1349,7 @@ int fused_moe_impl(const void* x, const void* gate, const void* up, const void* 
     }
     if (!w) return ws_fail("fused_moe", L.total, e);
     return run_moe(p, x, gate, up, down, reinterpret_cast<const float*>(rw), reinterpret_cast<const uint32_t*>(idx),
-                   out, overwrite, reinterpret_cast<char*>(w->ptr), s, f8, true);
+                   out, overwrite, reinterpret_cast<char*>(w->ptr), s, f8, true, mx);
 }
 
 // ----------------------------------------------- fused MoE without allocation

@@ -5,8 +5,6 @@
 #include <stddef.h>
 #include <stdint.h>
 
-#include <mutex>
-
 namespace cm {
 
 // ---------------------------------------------------------------- router
@@ -171,6 +169,10 @@ struct GemmArgs {
     // of B0 and (kGateUp) B1
     const float* scale0;
     const float* scale1;
+    // MXFP4 weights (launch_moe_gemm_mx): scale bytes [E][N][K/32] of B0 and
+    // (kGateUp) B1, 4-byte aligned; codes [E][N][K/2], strideB = N * K, ldb = K
+    const uint8_t* mx0;
+    const uint8_t* mx1;
     // 32-row kernel, kFc1 / kDown / kFc2 with 16-bit weights: 128-column
     // tiles instead of 256 (n_tiles counts those)
     int narrow;
@@ -302,6 +304,10 @@ hipError_t launch_moe_gemm_lds(int mode, int dtype, int cfg, const GemmArgs& a, 
 // kFc1, kDown, kFc2.
 // cfg: kW8Gemv or kLdsRows32 (decode), or kLds256w8
 hipError_t launch_moe_gemm_w8(int mode, int dtype, int cfg, const GemmArgs& a, hipStream_t stream);
+// GEMMs over MXFP4 weights: kGateUp, kFc1, kDownRows / kFc2Rows (C: f32 rows
+// [T*k, N] by pair, unweighted), kDownSet / kFc2Set; cfg kLdsRows32 (not the
+// sets), kLds128, kLds128x256o2 or kLds256w8
+hipError_t launch_moe_gemm_mx(int mode, int dtype, int cfg, const GemmArgs& a, hipStream_t stream);
 // kW8Gemv (moe_gemv_w8.hip): modes kGateUp, kFc1, kDown, kFc2 (pair path,
 // f32 atomics for kDown / kFc2)
 hipError_t launch_w8_gemv(int mode, int dtype, const GemmArgs& a, hipStream_t stream);
@@ -397,6 +403,9 @@ hipError_t launch_fill_zero_bytes(void* p, long long nbytes, hipStream_t stream)
 // slots whose expert idx[t*k + j] >= E were dropped and have no row)
 hipError_t launch_pair_rows_sum(void* out, int dtype, const void* rows, const uint32_t* idx, int E, int T, int k,
                                 int H, bool overwrite, hipStream_t stream);
+// the same over unweighted f32 rows: out[t] = dtype(out[t] + sum_j w[t,j] * rows[t*k + j])
+hipError_t launch_pair_rows32_sum(void* out, int dtype, const float* rows, const float* w, const uint32_t* idx, int E,
+                                  int T, int k, int H, bool overwrite, hipStream_t stream);
 // out[i] = dtype(out[i] + acc[i]), or dtype(acc[i]) with overwrite
 hipError_t launch_finalize(void* out, int dtype, const float* acc, long long n, bool overwrite, hipStream_t stream);
 
@@ -405,27 +414,16 @@ hipError_t launch_finalize(void* out, int dtype, const float* acc, long long n, 
 int set_error(int code, const char* fmt, ...);
 void clear_error();
 int hip_fail(hipError_t e, const char* what);
-int cus_per_xcd();  // CUs of the current device over its 8 XCDs, 0 if unknown
-// Decode GEMMs: workgroups of one round; columns per lane (capi.hip)
-int dec_cap();
-int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32, int most = 8);
-// The library-owned workspace of (current device, s), held until `lock` goes.
-// need: bytes a call takes; reserve (>= need): bytes to have for the calls to come.
-struct WsLease {
-    std::unique_lock<std::mutex> lock;
-    char* ptr = nullptr;
-    size_t bytes = 0;
-};
-int lease_workspace(const char* who, size_t need, size_t reserve, hipStream_t s, WsLease& l);
-// Workspace of fused_moe over pre-packed 16-bit weights for every batch up to T
-// tokens (aligned operands); 0 with the error set where the sizes are refused.
-size_t packed_upto_bytes(int T, int H, int I, int E, int k, int act, uint32_t moe_type, uint32_t dtype);
 int topk_softmax_impl(const void* g, int gdt, void* w, int wdt, void* idx, void* ei, int E, int T, int k,
                       void* stream);
 struct Fp8Weights;
+// MXFP4 weights' scale bytes, and those of MXFP8 rows (null: 16-bit rows)
+struct MxWeights {
+    const uint8_t *gate_s, *up_s, *down_s, *x_s;
+};
 int fused_moe_impl(const void* x, const void* gate, const void* up, const void* down, const void* rw,
                    const void* idx, void* out, int T, int H, int I, int E, int k, int act, uint32_t moe_type,
                    uint32_t dtype, void* ws, size_t ws_bytes, bool own_ws, bool overwrite, void* stream,
-                   const Fp8Weights* f8 = nullptr, bool packed = false);
+                   const Fp8Weights* f8 = nullptr, bool packed = false, const MxWeights* mx = nullptr);
 
 }  // namespace cm

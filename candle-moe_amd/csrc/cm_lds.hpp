@@ -50,6 +50,14 @@ __device__ __forceinline__ void dma16s(const i32x4& r, uint32_t lds_off, uint32_
                  : "memory");
 }
 
+// 64 lanes x 4 bytes into LDS at lds_off + 4*lane (4-byte aligned offsets).
+__device__ __forceinline__ void dma4(const i32x4& r, uint32_t lds_off, uint32_t voff) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds_off), "v"(voff), "s"(r)
+                 : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void wait_vm() {
     static_assert(N >= 0 && N < 64, "vmcnt range");
@@ -81,6 +89,13 @@ template <int ACH>
 __device__ __forceinline__ int a_swz(int r, int c) {
     if constexpr (ACH == 8) return (c ^ r ^ (r >> 3)) & 7;
     else return (c ^ (r >> 2)) & 3;
+}
+
+// Rows of 4-bit codes (KCH chunks of 32 k): a lane reads one 16-byte chunk of its
+// row; rows 32 bytes apart, so of 16 rows the second eight swap their chunks.
+template <int KCH>
+__device__ __forceinline__ int w4_swz(int r, int c) {
+    return KCH == 2 ? c ^ ((r >> 3) & 1) : c;
 }
 
 // [K,N] sub-tile rows of BCH 16-byte chunks: chunk c of k-row r is stored at
@@ -490,6 +505,28 @@ __device__ __forceinline__ void tile_epilogue(const GemmArgs& a, f32x16 (&acc)[M
                 }
             }
         }
+    }
+}
+
+// Pair rows in f32, unweighted (MXFP4 weights): rows[dst] = acc, dst the pair of
+// this lane's row in each block (the swapped layout: 4 consecutive columns).
+template <int BN, int WM, int WN, int MB, int NB>
+__device__ __forceinline__ void rows32_epilogue(const GemmArgs& a, f32x16 (&acc)[MB][NB], int m_valid, int nt, int wm,
+                                                int wn, int lane, const int* dst) {
+    const int N = a.N, lr = lane & 31, nsub = 4 * (lane >> 5);
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        if (wm * WM + mb * 32 + lr >= m_valid) continue;
+        float* C = reinterpret_cast<float*>(a.C) + (long long)dst[mb] * N;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = nt * BN + wn * WN + nb * 32 + 8 * g + nsub;
+                if (col >= N) continue;
+                *reinterpret_cast<f32x4*>(C + col) = f32x4{acc[mb][nb][4 * g], acc[mb][nb][4 * g + 1],
+                                                           acc[mb][nb][4 * g + 2], acc[mb][nb][4 * g + 3]};
+            }
     }
 }
 

@@ -601,6 +601,54 @@ hipError_t launch_pair_rows_sum(void* out, int dtype, const void* rows, const ui
     return hipGetLastError();
 }
 
+// Unweighted f32 pair rows -> token rows: one thread per 4 consecutive columns
+// of a token, up to 4 of its rows in flight (in slot order: the same bits always).
+template <int DT>
+__global__ __launch_bounds__(256) void pair_rows32_sum_k(uint16_t* __restrict__ out, const float* __restrict__ rows,
+                                                         const float* __restrict__ w, const uint32_t* __restrict__ idx,
+                                                         int E, int T, int k, int H, int overwrite) {
+    const int h4 = H / 4;
+    const long long n = (long long)T * h4;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        const long long t = i / h4, c = (i - t * h4) * 4;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!overwrite) {
+            const u32x2 o = *reinterpret_cast<const u32x2*>(out + t * H + c);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[q] = Elem<DT>::to_f32((uint16_t)((o[q >> 1] >> (16 * (q & 1))) & 0xffffu));
+        }
+        for (int j0 = 0; j0 < k; j0 += 4) {
+            f32x4 v[4];
+            float wj[4];
+            bool ok[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const long long p = t * k + min(j0 + j, k - 1);
+                ok[j] = j0 + j < k && idx[p] < (uint32_t)E;  // (a dropped pair has no row)
+                wj[j] = w[p];
+                v[j] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(rows + p * H + c));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) s[q] = ok[j] ? fmaf(wj[j], v[j][q], s[q]) : s[q];
+        }
+        *reinterpret_cast<u32x2*>(out + t * H + c) = u32x2{pack2<DT>(s[0], s[1]), pack2<DT>(s[2], s[3])};
+    }
+}
+
+hipError_t launch_pair_rows32_sum(void* out, int dtype, const float* rows, const float* w, const uint32_t* idx, int E,
+                                  int T, int k, int H, bool overwrite, hipStream_t stream) {
+    if (T <= 0 || H <= 0) return hipSuccess;
+    if ((dtype != kBF16 && dtype != kF16) || H % 4) return hipErrorInvalidValue;
+    const dim3 g(grid_for((long long)T * (H / 4), 256)), b(256);
+    uint16_t* o = reinterpret_cast<uint16_t*>(out);
+    const int ow = overwrite ? 1 : 0;
+    if (dtype == kBF16) hipLaunchKernelGGL(pair_rows32_sum_k<kBF16>, g, b, 0, stream, o, rows, w, idx, E, T, k, H, ow);
+    else hipLaunchKernelGGL(pair_rows32_sum_k<kF16>, g, b, 0, stream, o, rows, w, idx, E, T, k, H, ow);
+    return hipGetLastError();
+}
+
 hipError_t launch_finalize(void* out, int dtype, const float* acc, long long n, bool overwrite, hipStream_t stream) {
     if (n <= 0) return hipSuccess;
     const dim3 g(grid_for(n, 256)), b(256);

@@ -49,8 +49,15 @@ using namespace lds;
 // / 165 -> 283 / 158 us. Not on the 256x256 kernel: its extended tiles took 13 %
 // longer, which the fewer tiles repaid only here and there (Qwen3 T=4096 203 /
 // 136 -> 213 / 122, Nomic T=8191 112 / 80 -> 115 / 79 us).
+// W4: MXFP4 weights ([N,K/2] codes, [N,K/32] scale bytes per expert). A B row of a
+// stage is BK / 2 bytes of codes, and a column's scales come as the one or two
+// aligned dwords that hold the tile's bytes (rows of K / 32 bytes start anywhere).
+// The products take the k of a tile in another order: lane half h holds the KSTEPS
+// chunks of 8 from h * KSTEPS on, so that its codes of the whole tile are one LDS
+// read and (BK 64) belong to one scale; the A fragments follow. The scaled
+// conversion makes each operand right before its MFMAs.
 template <int DT, int BM, int BN, int BK, int NST, int NW, int MODE, int WGM = 2, int OCC = 1, bool W8 = false,
-          bool PK = false, int EXT = 0>
+          bool PK = false, int EXT = 0, bool W4 = false>
 __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     // NW waves in WGM rows: 4 in a 2x2 layout (one per SIMD), 8 in 2x4 (two
     // per SIMD, so one wave's MFMAs cover the other's LDS, DMA and VALU work),
@@ -68,7 +75,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     // KC: 16-bit weights stored K-contiguous ([N,K] per expert): Nomic's fc2
     // in the API layout, or every GEMM on pre-packed weights (PK)
     constexpr bool KC = BNK || PK;
-    static_assert(!(W8 && PK), "fp8 codes are K-contiguous already");
+    static_assert(!(W8 && PK) && !(W4 && (W8 || PK || BNK)), "codes are K-contiguous already");
     constexpr bool ROWS = (MODE == kDownRows || MODE == kFc2Rows);
     constexpr bool ATOMIC = (MODE == kDown || MODE == kFc2);
     constexpr bool SWAP = !ATOMIC;
@@ -80,20 +87,25 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     constexpr int A_BYTES = BM * AROW;
     // W8: fp8 e4m3 weights, K-contiguous ([N,K] per expert, one byte per
     // element), each n-row of a B sub-tile BK bytes of KCH 16-byte chunks
-    constexpr int KROW = BK;
+    constexpr int KROW = W4 ? BK / 2 : BK;
     constexpr int KCH = KROW / 16;
-    constexpr int KRPI = 1024 / KROW;  // fp8 n-rows per DMA instruction
-    constexpr int B_BYTES = W8 ? BN * KROW : BN * AROW;
+    constexpr int KRPI = 1024 / KROW;  // n-rows of codes per DMA instruction
+    constexpr int B_BYTES = W8 || W4 ? BN * KROW : BN * AROW;
+    constexpr int SDW = BK / 32;       // W4: scale dwords per column and stage
+    constexpr int S_BYTES = W4 ? BN * 4 * SDW : 0;
+    constexpr int S_INS = S_BYTES / (256 * NW);  // (one dword per lane)
+    static_assert(S_INS * 256 * NW == S_BYTES, "scale DMA split");
     static_assert(EXT == 0 || (EXT == 32 && NW == 4 && BM == 128 && WGM == 2 && NB % 2 == 0 && !ATOMIC && !W8),
                   "extended tiles");
     constexpr bool EX = EXT > 0;
     constexpr int NX = EX ? NB / 2 : 1;     // column blocks of the extension rows per wave
     constexpr int X_INS = EX ? EXT / RPA : 1;  // DMA instructions of the extension rows (per stage)
-    constexpr int X_OFF = A_BYTES + B_BYTES;
-    constexpr int STAGE = A_BYTES + B_BYTES + EXT * AROW;
+    constexpr int X_OFF = A_BYTES + B_BYTES + S_BYTES;
+    constexpr int STAGE = X_OFF + EXT * AROW;
     constexpr int A_INS = A_BYTES / (1024 * NW);  // DMA instructions per wave per stage
     constexpr int B_INS = B_BYTES / (1024 * NW);
-    constexpr int LOADS = A_INS + B_INS;
+    constexpr int LOADS = A_INS + B_INS + S_INS;
+    static_assert(!W4 || B_INS * 1024 * NW == B_BYTES, "code DMA split");
     // [K,N] weights: gate and up (DUAL) get separate sub-tiles, so that every
     // DMA instruction reads one tensor through one (uniform) buffer resource.
     constexpr int NSUB = DUAL ? 2 : 1;
@@ -103,10 +115,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     constexpr int RPI = 1024 / BROW;       // k-rows per DMA instruction
     constexpr int SUB_BYTES = BK * BROW;
     constexpr int SUB_INS = SUB_BYTES / (1024 * NW);  // per wave, per sub-tile
-    static_assert(A_INS * 1024 * NW == A_BYTES && SUB_INS * 1024 * NW == SUB_BYTES, "DMA split");
+    static_assert(A_INS * 1024 * NW == A_BYTES && (W4 || SUB_INS * 1024 * NW == SUB_BYTES), "DMA split");
     static_assert(!DUAL || (WN % 64) == 0, "gate/up pairs must stay inside one wave");
     static_assert(KC || BCH >= 8, "[K,N] tiles need >= 8 chunks per row for the swizzle");
-    static_assert(KC || W8 || SUB_INS * NSUB == B_INS, "B tile split");
+    static_assert(KC || W8 || W4 || SUB_INS * NSUB == B_INS, "B tile split");
+    static_assert(!W4 || SUBN % KRPI == 0, "a DMA instruction reads one tensor's codes");
     // K-contiguous 16-bit sub-tiles (gate / up apart for DUAL): SUBN n-rows of
     // AROW bytes each
     constexpr int KSUB_BYTES = SUBN * AROW;
@@ -117,7 +130,13 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     static_assert(!W8 || (!BNK && KCH == 4 && W8_SUB_INS * 1024 * NW == W8_SUB_BYTES && W8_SUB_INS * NSUB == B_INS),
                   "fp8 B tile");
     static_assert(LOADS * (NST - 2) < 64, "vmcnt range");
-    __shared__ __attribute__((aligned(1024))) char smem[NST * STAGE];
+    // staged (row-contiguous) epilogue of the large tiles, see staged_epilogue
+    constexpr bool R32 = W4 && ROWS;  // f32 pair rows, unweighted (summed with the weights afterwards)
+    constexpr bool STAGED = SWAP && BM >= 128 && !R32;
+    constexpr int OUT_BYTES = STAGED ? BM * (DUAL ? BN / 2 : BN) * 2 : 0;
+    static_assert(!STAGED || W4 || NST * STAGE >= OUT_BYTES, "output tile fits the stages");
+    constexpr int SMEM = NST * STAGE > OUT_BYTES ? NST * STAGE : OUT_BYTES;
+    __shared__ __attribute__((aligned(1024))) char smem[SMEM];
     __shared__ int32_t s_tok[(ATOMIC || SET) ? BM + EXT : 1];
     __shared__ float s_w[ATOMIC ? BM : 1];
     __shared__ float s_sc[W8 ? BN : 1];
@@ -125,10 +144,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     // column scale, or 1 for an all-zero column), [kSetMaxK][BN]
     constexpr bool W8SET = W8 && SET;
     __shared__ __attribute__((aligned(16))) float s_unit[W8SET ? kSetMaxK * BN : 4];
-    // staged (row-contiguous) epilogue of the large tiles, see staged_epilogue
-    constexpr bool STAGED = SWAP && BM >= 128;
-    static_assert(!STAGED || NST * STAGE >= BM * (DUAL ? BN / 2 : BN) * 2, "output tile fits the stages");
-    __shared__ int32_t s_dst[STAGED ? BM + EXT : 1];
+    __shared__ int32_t s_dst[STAGED || (R32 && EX) ? BM + EXT : 1];
     __shared__ float s_wx[EX ? EXT : 1];  // routing weights of the extension rows
 
     // workgroup -> (output tile, K split); every workgroup first clears its
@@ -222,7 +238,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     uint32_t b_off[B_INS];
 #pragma unroll
     for (int i = 0; i < B_INS; ++i) {
-        if constexpr (W8) {
+        if constexpr (W4) {
+            // n-row r of the tile's BN (gate's SUBN, then up's for DUAL)
+            const int r = KRPI * (NW * i + wave) + lane / KCH;
+            const int n = nt * SUBN + r % SUBN;
+            b_off[i] = n < N ? (uint32_t)n * (uint32_t)(a.ldb / 2) + (uint32_t)(w4_swz<KCH>(r, lane % KCH) * 16) : kOob;
+        } else if constexpr (W8) {
             // n-row r of sub-tile i / W8_SUB_INS; the lane's slot receives the
             // chunk a_swz(r, slot) of that row (byte offsets: one byte per k)
             const int q = NW * (i % W8_SUB_INS) + wave;
@@ -245,6 +266,17 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
         }
     }
 
+    // W4: first scale byte of this lane's column, which instruction i fetches dword
+    // lane % SDW of
+    uint32_t s_off[S_INS > 0 ? S_INS : 1];
+    if constexpr (W4) {
+#pragma unroll
+        for (int i = 0; i < S_INS; ++i) {
+            const int n = nt * SUBN + (64 * (NW * i + wave) + lane) / SDW % SUBN;
+            s_off[i] = n < N ? (uint32_t)n * (uint32_t)(a.ldb / 32) : kOob;
+        }
+    }
+
     // fp8 weights: this thread's column scale of the tile (256 threads, 256
     // columns: gate then up for kGateUp), loaded now, staged in LDS for the
     // epilogue after the K loop
@@ -260,12 +292,20 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     // the expert changes every seg_len of K (tracked as K advances, issue
     // calls come in increasing k0).
     int seg = 0, seg_k0 = 0;
+    i32x4 rS0, rS1;  // (W4: of its scale bytes)
     auto weights_rsrc = [&](int e, i32x4& r0s, i32x4& r1s) {
-        constexpr int BES = W8 ? 1 : 2;  // bytes per weight element
-        const long long eoff = (long long)e * a.strideB * BES;
-        r0s = make_rsrc(reinterpret_cast<const char*>(a.B0) + eoff, a.strideB * BES);
+        // bytes per expert's matrix
+        const long long eb = W4 ? a.strideB / 2 : a.strideB * (W8 ? 1 : 2);
+        const long long eoff = (long long)e * eb;
+        r0s = make_rsrc(reinterpret_cast<const char*>(a.B0) + eoff, eb);
         r1s = r0s;
-        if constexpr (DUAL) r1s = make_rsrc(reinterpret_cast<const char*>(a.B1) + eoff, a.strideB * BES);
+        if constexpr (DUAL) r1s = make_rsrc(reinterpret_cast<const char*>(a.B1) + eoff, eb);
+        if constexpr (W4) {
+            const long long sb = a.strideB / 32;
+            rS0 = make_rsrc(a.mx0 + (long long)e * sb, sb);
+            rS1 = rS0;
+            if constexpr (DUAL) rS1 = make_rsrc(a.mx1 + (long long)e * sb, sb);
+        }
     };
     i32x4 rB0, rB1;
     weights_rsrc(seg_exp[0], rB0, rB1);
@@ -290,7 +330,19 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
         // a tile that lies inside the operands in K takes the SGPR-offset path;
         // a K tail checks every lane's chunk against K
         const uint32_t sa = (uint32_t)k0 * 2u;
-        const uint32_t sb = W8 ? (uint32_t)kk : (KC ? (uint32_t)kk * 2u : (uint32_t)kk * (uint32_t)a.ldb * 2u);
+        if constexpr (W4) {
+            // scales: the aligned dwords around the tile's bytes
+#pragma unroll
+            for (int i = 0; i < S_INS; ++i) {
+                if (A_INS + B_INS + i < lo || A_INS + B_INS + i >= hi) continue;
+                const int q = NW * i + wave;
+                const bool up = DUAL && 64 * q >= SUBN * SDW;
+                const uint32_t o = s_off[i] == kOob ? kOob
+                                                    : ((s_off[i] + (uint32_t)(kk / 32)) & ~3u) + 4u * (lane % SDW);
+                dma4(up ? rS1 : rS0, sB + B_BYTES + q * 256, o);
+            }
+        }
+        const uint32_t sb = W4 ? (uint32_t)kk / 2u : W8 ? (uint32_t)kk : (KC ? (uint32_t)kk * 2u : (uint32_t)kk * (uint32_t)a.ldb * 2u);
         if (k0 + BK <= K && kk + BK <= klim) {
             // the tile lies inside the operands in K: one SGPR offset for all lanes
 #pragma unroll
@@ -299,7 +351,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
 #pragma unroll
             for (int i = 0; i < B_INS; ++i) {
                 if (A_INS + i < lo || A_INS + i >= hi) continue;
-                if constexpr (W8) {
+                if constexpr (W4) {
+                    const int q = NW * i + wave;
+                    dma16s(DUAL && KRPI * q >= SUBN ? rB1 : rB0, sB + q * 1024, b_off[i], sb);
+                } else if constexpr (W8) {
                     const int sub = i / W8_SUB_INS;
                     dma16s(sub ? rB1 : rB0, sB + sub * W8_SUB_BYTES + (NW * (i % W8_SUB_INS) + wave) * 1024, b_off[i],
                            sb);
@@ -332,7 +387,13 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
 #pragma unroll
             for (int i = 0; i < B_INS; ++i) {
                 if (A_INS + i < lo || A_INS + i >= hi) continue;
-                if constexpr (W8) {
+                if constexpr (W4) {
+                    // (K is a multiple of 32: likewise)
+                    const int q = NW * i + wave;
+                    const int r = KRPI * q + lane / KCH;
+                    const bool in = kk + w4_swz<KCH>(r, lane % KCH) * 32 < klim;
+                    dma16s(DUAL && KRPI * q >= SUBN ? rB1 : rB0, sB + q * 1024, in ? b_off[i] : kOob, sb);
+                } else if constexpr (W8) {
                     // (K is a multiple of 16: a chunk lies wholly inside or outside)
                     const int sub = i / W8_SUB_INS;
                     const int r = KRPI * (NW * (i % W8_SUB_INS) + wave) + lane / KCH;
@@ -441,7 +502,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     };
     // the extension rows' A fragment of one k16 step, and its MFMAs
     auto load_x = [&](const char* sA, int kk, u32x4& xf) {
-        xf = *reinterpret_cast<const u32x4*>(sA + X_OFF + lr * AROW + a_swz<ACH>(lr, kk * 2 + lh) * 16);
+        const int c = W4 ? lh * KSTEPS + kk : kk * 2 + lh;
+        xf = *reinterpret_cast<const u32x4*>(sA + X_OFF + lr * AROW + a_swz<ACH>(lr, c) * 16);
     };
     auto mfma_x = [&](const u32x4& xf, const u32x4 (&bfr)[NB]) {
 #pragma unroll
@@ -483,7 +545,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     };
     // LDS read instructions per k16 step (ds_read_b128 for A and [N,K] B,
     // two ds_read_b64_tr_b16 per [K,N] B block).
-    constexpr int DS_PER_STEP = MB + ((KC || W8) ? NB : 2 * NB);
+    constexpr int DS_PER_STEP = MB + (W4 ? 0 : (KC || W8) ? NB : 2 * NB);
     constexpr int MFMA_PER_STEP = MB * NB;
     // Pin the schedule of one region: one MFMA, then one LDS read, while
     // reads remain, then the remaining MFMAs (masks: 0x8 MFMA, 0x100 DS read).
@@ -653,6 +715,67 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
         dma_slice(ds, dk, KSTEPS - 1);
     };
 
+    // MXFP4 weights: the codes of the tile and their scales first, then step by step
+    // the A fragments of the next step under the conversions and MFMAs of this one.
+    // kk0: the tile's first k in the weight rows, klim: their k
+    auto compute_w4 = [&](auto x, int stage, int ds, int dk, int kk0, int klim) {
+        constexpr bool X = decltype(x)::value;
+        if (!rows_live) {
+#pragma unroll
+            for (int st = 0; st < KSTEPS; ++st) dma_slice(ds, dk, st);
+            return;
+        }
+        const char* sA = smem + stage * STAGE;
+        const char* sB = sA + A_BYTES;
+        const char* sS = sB + B_BYTES;
+        u32x4 af[2][MB], bfr[NB], xf;
+        uint32_t braw[NB][KSTEPS];
+        float sc[NB];
+        auto load_a = [&](int kk) {
+            const int c = lh * KSTEPS + kk;
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) {
+                const int r = a_frag_row[mb];
+                af[kk & 1][mb] = *reinterpret_cast<const u32x4*>(sA + r * AROW + a_swz<ACH>(r, c) * 16);
+            }
+        };
+        load_a(0);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = (DUAL ? (nb & 1) * SUBN + wn * (WN / 2) + (nb >> 1) * 32 : wn * WN + nb * 32) + lr;
+            const uint32_t first = (uint32_t)(nt * SUBN + r % SUBN) * (uint32_t)(a.ldb / 32) + (uint32_t)(kk0 / 32);
+            if constexpr (BK == 64) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(sB + r * KROW + w4_swz<KCH>(r, lh) * 16);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) braw[nb][q % KSTEPS] = v[q];
+                const uint64_t d = *reinterpret_cast<const uint64_t*>(sS + r * 8);
+                uint32_t e = (uint32_t)(d >> (8u * ((first & 3u) + (uint32_t)lh))) & 255u;
+                // (past K: the codes are zeros, a foreign scale could be a NaN)
+                if (kk0 + 32 * lh >= klim) e = 127u;
+                sc[nb] = __uint_as_float(e << 23);
+            } else {
+                const u32x2 v = *reinterpret_cast<const u32x2*>(sB + r * KROW + lh * 8);
+                braw[nb][0] = v[0];
+                braw[nb][KSTEPS - 1] = v[1];
+                const uint32_t d = *reinterpret_cast<const uint32_t*>(sS + r * 4);
+                sc[nb] = __uint_as_float(((d >> (8u * (first & 3u))) & 255u) << 23);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) {
+            if (kk + 1 < KSTEPS) load_a(kk + 1);
+            if constexpr (X) load_x(sA, kk, xf);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) bfr[nb] = mx4x8_to<DT>(braw[nb][kk], sc[nb]);
+            mfma_step(af[kk & 1], bfr);
+            if constexpr (X) mfma_x(xf, bfr);
+            if (kk + 1 < KSTEPS) interleave(x);
+            __builtin_amdgcn_sched_barrier(0);
+            dma_slice(ds, dk, kk);
+        }
+    };
+
     if constexpr (ATOMIC) {
         if (tid < BM) {
             const int p = a.sorted_pair[r0 + (tid < m_valid ? tid : 0)];
@@ -707,7 +830,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     const int nk = min(nk_all, kt0 + per_split) - kt0;
 
     if (nk > 0) issue(0, kt0 * BK, false);
-    if constexpr (NW == 4 && !GATHER && !W8) {
+    if constexpr (NW == 4 && !GATHER && !W8 && !W4) {
         // 4-wave down / fc2 kernels: hand-over one k16 step early. The
         // barrier of tile kt+1 sits before the MFMAs of tile kt's last k16
         // step, whose fragments are already in registers, so the MFMAs issued
@@ -823,7 +946,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
                 seg_next += seg_kt;
             }
         }
-        if constexpr (W8 && NW == 8 && KSTEPS == 4)
+        if constexpr (W4) {
+            const int klim = SET ? a.seg_len : K;
+            const int kk0 = SET ? (kt0 + kt) * BK % a.seg_len : (kt0 + kt) * BK;
+            compute_w4(x, kt % NST, (late && ahead < nk) ? ahead % NST : -1, (kt0 + ahead) * BK, kk0, klim);
+        } else if constexpr (W8 && NW == 8 && KSTEPS == 4)
             compute_w8i(kt % NST, (late && ahead < nk) ? ahead % NST : -1, (kt0 + ahead) * BK);
         else if constexpr (W8) compute_w8(kt % NST);
         else compute(x, kt % NST, (late && ahead < nk) ? ahead % NST : -1, (kt0 + ahead) * BK);
@@ -870,6 +997,20 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
         }
     }
     const int m_tile = EX ? min(m_valid, BM) : m_valid;  // the tile's own rows
+    if constexpr (R32) {
+        rows32_epilogue<BN, WM, WN, MB, NB>(a, acc, m_tile, nt, wm, wn, lane, pre_dst);
+        if constexpr (EX) {
+            if (ext_rows) {
+                __syncthreads();  // (stage_x_rows ran on one wave)
+                f32x16 blk[1][NX];
+#pragma unroll
+                for (int j = 0; j < NX; ++j) blk[0][j] = accx[j];
+                const int dst[1] = {s_dst[BM + lr]};
+                rows32_epilogue<BN, 32, NX * 32, 1, NX>(a, blk, m_valid - BM, nt, 0, 2 * wn + wm, lane, dst);
+            }
+        }
+        return;
+    }
     if constexpr (STAGED) {
         if (!SET || a.overwrite) {
             // output row of every tile row (gate/up, fc1: the pair's inter row;
@@ -881,12 +1022,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
                 }
             }
             __syncthreads();  // every wave is done with the stages
-            staged_epilogue<DT, MODE, BM, BN, WM, WN, MB, NB, NW, W8 && !SET, EXT, NST * STAGE, NX>(
+            staged_epilogue<DT, MODE, BM, BN, WM, WN, MB, NB, NW, W8 && !SET, EXT, SMEM, NX>(
                 a, acc, smem, SET ? s_tok : s_dst, EX ? m_valid : m_tile, nt, wm, wn, lane, pre_w, sc0, sc1, accx,
                 s_wx);
             return;
         }
-        if constexpr (SET && BN == 256 && NST * STAGE >= BM * (BN / 2) * 4) {
+        if constexpr (SET && BN == 256 && SMEM >= BM * (BN / 2) * 4) {
             __syncthreads();  // every wave is done with the stages
             staged_epilogue_acc<DT, BM, BN, WM, WN, MB, NB, NW>(a, acc, smem, s_tok, m_tile, nt, wm, wn, lane);
             return;
@@ -983,6 +1124,68 @@ static hipError_t launch_w8_mode(int cfg, const GemmArgs& a, hipStream_t stream)
                        dim3(256), 0, stream, a);
     return hipGetLastError();
 }
+// MXFP4 weights: gate/up, fc1, f32 pair rows and expert sets
+template <int DT, int MODE>
+static hipError_t launch_mx_mode(int cfg, const GemmArgs& a, hipStream_t stream) {
+    const long long tiles = (long long)a.m_tiles_max * a.n_tiles;
+    const long long nwg_l = a.tail_cus > 0 ? 8 * ((tiles + 7) / 8 + a.tail_cus) : split_grid(tiles, a);
+    if (nwg_l > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (nwg_l <= 0) return hipSuccess;
+    if (a.ext != 0 && ext_rows_of(cfg) != a.ext) return hipErrorInvalidValue;
+    const dim3 g((unsigned)nwg_l);
+    constexpr int X = kTileExt;
+    switch (cfg) {
+        case kLds128:
+            hipLaunchKernelGGL((moe_lds_gemm<DT, 128, 128, 64, 4, 4, MODE, 2, 1, false, false, X, true>), g, dim3(256), 0,
+                               stream, a);
+            break;
+        case kLds256w8:
+            hipLaunchKernelGGL((moe_lds_gemm<DT, 256, 256, 64, 3, 8, MODE, 2, 1, false, false, 0, true>), g, dim3(512), 0,
+                               stream, a);
+            break;
+        case kLds128x256o2:
+            hipLaunchKernelGGL((moe_lds_gemm<DT, 128, 256, 32, 3, 4, MODE, 2, 2, false, false, X, true>), g, dim3(256), 0,
+                               stream, a);
+            break;
+        case kLdsRows32:
+            if constexpr (MODE != kDownSet) {
+                if constexpr (MODE != kGateUp) {
+                    if (a.narrow) {
+                        hipLaunchKernelGGL((moe_lds_gemm<DT, 32, 128, 64, 4, 4, MODE, 1, 1, false, false, 0, true>), g,
+                                           dim3(256), 0, stream, a);
+                        break;
+                    }
+                }
+                hipLaunchKernelGGL((moe_lds_gemm<DT, 32, 256, 64, 4, 4, MODE, 1, 1, false, false, 0, true>), g, dim3(256),
+                                   0, stream, a);
+                break;
+            }
+            return hipErrorInvalidValue;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+template <int DT>
+static hipError_t launch_mx_dt(int mode, int cfg, const GemmArgs& a, hipStream_t stream) {
+    // [N,K] codes for every GEMM: fc2 (Nomic) runs the down kernels
+    switch (mode) {
+        case kGateUp: return launch_mx_mode<DT, kGateUp>(cfg, a, stream);
+        case kFc1: return launch_mx_mode<DT, kFc1>(cfg, a, stream);
+        case kDownRows:
+        case kFc2Rows: return launch_mx_mode<DT, kDownRows>(cfg, a, stream);
+        case kDownSet:
+        case kFc2Set: return launch_mx_mode<DT, kDownSet>(cfg, a, stream);
+        default: return hipErrorInvalidValue;
+    }
+}
+hipError_t launch_moe_gemm_mx(int mode, int dtype, int cfg, const GemmArgs& a, hipStream_t stream) {
+    if (a.mx0 == nullptr || (mode == kGateUp && a.mx1 == nullptr) || a.ldb % 32 || a.strideB % 32)
+        return hipErrorInvalidValue;
+    if (dtype == kBF16) return launch_mx_dt<kBF16>(mode, cfg, a, stream);
+    if (dtype == kF16) return launch_mx_dt<kF16>(mode, cfg, a, stream);
+    return hipErrorInvalidValue;
+}
+
 template <int DT>
 static hipError_t launch_w8_dt(int mode, int cfg, const GemmArgs& a, hipStream_t stream) {
     // [N,K] fp8 weights for every GEMM: fc2 (Nomic) runs the down kernels

@@ -24,116 +24,6 @@ struct MxCall {
     bool accumulate;
 };
 
-constexpr size_t kMxHeader = 256;  // the workspaces' own counters
-
-// Every weight matrix in 16 bits, then the pre-packed path over them.
-static int run_mx_expanded(const MxCall& c, hipStream_t s) {
-    const bool qwen3 = c.moe_type == 0;
-    const size_t mat = a256_bytes((size_t)c.E * c.H * c.I * 2);
-    const size_t rows = c.x_scale ? a256_bytes((size_t)c.T * c.H * 2) : 0;
-    const size_t moe = packed_upto_bytes(c.T, c.H, c.I, c.E, c.k, c.act, c.moe_type, c.dtype);
-    if (moe == 0) return CANDLE_MOE_ERR_UNSUPPORTED;  // (the error is set)
-    const size_t need = kMxHeader + (qwen3 ? 3 : 2) * mat + rows + moe;
-    WsLease l;
-    const int rc = lease_workspace("fused_moe_mxfp4", need, need, s, l);
-    if (rc) return rc;
-    char* p = l.ptr + kMxHeader;
-    auto take = [&](size_t n) {
-        char* q = p;
-        p += n;
-        return q;
-    };
-    void* gate = take(mat);
-    void* up = take(mat);
-    void* down = qwen3 ? take(mat) : nullptr;
-    const void* x = c.x;
-    hipError_t e = launch_dequantize_mxfp4(c.gate, c.gate_s, c.E, c.I, c.H, gate, (int)c.dtype, s);
-    if (e == hipSuccess)
-        e = launch_dequantize_mxfp4(c.up, c.up_s, c.E, qwen3 ? c.I : c.H, qwen3 ? c.H : c.I, up, (int)c.dtype, s);
-    if (e == hipSuccess && qwen3) e = launch_dequantize_mxfp4(c.down, c.down_s, c.E, c.H, c.I, down, (int)c.dtype, s);
-    if (e == hipSuccess && c.x_scale) {
-        void* xr = take(rows);
-        e = launch_rows8_to(c.x, c.x_scale, c.T, c.H, xr, (int)c.dtype, s);
-        x = xr;
-    }
-    if (e != hipSuccess) return hip_fail(e, "fused_moe_mxfp4 dequantize");
-    return fused_moe_impl(x, gate, up, down, c.rw, c.idx, c.out, c.T, c.H, c.I, c.E, c.k, c.act, c.moe_type, c.dtype, p,
-                          moe, false, !c.accumulate, s, nullptr, true);
-}
-
-// Decode batches (moe_gemv_dec.hip): the pairs grouped inside the GEMM kernels,
-// the 4-bit codes streamed once, f32 rows by pair, one sum per token.
-static size_t mx_dec_bytes(const MxCall& c) {
-    const size_t P = (size_t)c.T * c.k;
-    return kMxHeader + 256 + a256_bytes(P * c.I * 2) + a256_bytes(P * c.H * 4);
-}
-static int run_mx_dec(const MxCall& c, char* ws, hipStream_t s) {
-    const bool qwen3 = c.moe_type == 0;
-    const int P = c.T * c.k;
-    int* meta = reinterpret_cast<int*>(ws + kMxHeader);
-    char* inter = ws + kMxHeader + 256;
-    float* part = reinterpret_cast<float*>(inter + a256_bytes((size_t)P * c.I * 2));
-    DecArgs d = {};
-    d.A = c.x;
-    d.B0 = c.gate;
-    d.B1 = c.up;
-    d.C = inter;
-    d.part = part;
-    d.meta = meta;
-    d.idx = reinterpret_cast<const uint32_t*>(c.idx);
-    d.P = P;
-    d.E = c.E;
-    d.K = d.ldb = c.H;
-    d.N = c.I;
-    d.k_top = c.k;
-    d.act = c.act;
-    d.strideB = (long long)c.H * c.I;
-    d.w4 = 1;
-    d.mx0 = reinterpret_cast<const uint8_t*>(c.gate_s);
-    d.mx1 = reinterpret_cast<const uint8_t*>(c.up_s);
-    d.xs = reinterpret_cast<const uint8_t*>(c.x_scale);
-    d.a_bytes = (long long)c.T * c.H * (c.x_scale ? 1 : 2);
-    d.max_groups = std::min(P, c.E);
-    d.rows_max = std::min(P, c.T);
-    d.cap = dec_cap();
-    d.ks_lim = 1;
-    d.cpl = dec_cpl(d.max_groups, c.I, false, 1, false, d.rows_max > 16 ? 6 : 8);
-    d.nblk = cdiv(c.I, 16 * d.cpl);
-    hipError_t e = launch_dec_gemv(qwen3 ? kGateUp : kFc1, (int)c.dtype, d, s);
-    if (e != hipSuccess) return hip_fail(e, "fused_moe_mxfp4 decode gate/up GEMM");
-    DecArgs d2 = d;
-    d2.A = inter;
-    d2.B0 = qwen3 ? c.down : c.up;
-    d2.B1 = nullptr;
-    d2.C = nullptr;
-    d2.K = d2.ldb = c.I;
-    d2.N = c.H;
-    d2.mx0 = reinterpret_cast<const uint8_t*>(qwen3 ? c.down_s : c.up_s);
-    d2.mx1 = nullptr;
-    d2.xs = nullptr;
-    d2.a_bytes = (long long)P * c.I * 2;
-    d2.cpl = dec_cpl(d.max_groups, c.H, false, 1, false, d.rows_max > 16 ? 6 : 8);
-    d2.nblk = cdiv(c.H, 16 * d2.cpl);
-    e = launch_dec_gemv(kDownRows, (int)c.dtype, d2, s);
-    if (e != hipSuccess) return hip_fail(e, "fused_moe_mxfp4 decode down GEMM");
-    DecFinish f = {};
-    f.part = part;
-    f.meta = meta;
-    f.ks_lim = 1;
-    f.P = P;
-    f.N = c.H;
-    f.E = c.E;
-    f.T = c.T;
-    f.k_top = c.k;
-    f.idx = d.idx;
-    f.routing_w = reinterpret_cast<const float*>(c.rw);
-    f.out = c.out;
-    f.overwrite = c.accumulate ? 0 : 1;
-    e = launch_dec_finish(kDownRows, (int)c.dtype, f, s);
-    return e == hipSuccess ? CANDLE_MOE_OK : hip_fail(e, "fused_moe_mxfp4 row sums");
-}
-constexpr long long kMxDecPairs = 256;
-
 static int run_mx(const MxCall& c, hipStream_t s) {
     if (c.T < 0) return set_error(CANDLE_MOE_ERR_INVALID, "fused_moe_mxfp4: num_tokens must be >= 0 (got %d)", c.T);
     if (c.E < 1 || c.E > 4096)
@@ -167,13 +57,12 @@ static int run_mx(const MxCall& c, hipStream_t s) {
                          "fused_moe_mxfp4: input, weights and output must be 16-byte aligned");
     if ((long long)c.T * c.H * 2 >= lim || P * c.I * 2 >= lim || (long long)c.H * c.I * 2 >= lim)
         return set_error(CANDLE_MOE_ERR_UNSUPPORTED, "fused_moe_mxfp4: operands beyond 2 GiB");
-    if (P <= kMxDecPairs) {
-        WsLease l;
-        const size_t need = mx_dec_bytes(c);
-        const int rc = lease_workspace("fused_moe_mxfp4", need, need, s, l);
-        return rc ? rc : run_mx_dec(c, l.ptr, s);
-    }
-    return run_mx_expanded(c, s);
+    if (!aligned(c.gate_s, 4) || !aligned(c.up_s, 4) || (qwen3 && !aligned(c.down_s, 4)))
+        return set_error(CANDLE_MOE_ERR_UNSUPPORTED, "fused_moe_mxfp4: weight scales must be 4-byte aligned");
+    const MxWeights mx = {reinterpret_cast<const uint8_t*>(c.gate_s), reinterpret_cast<const uint8_t*>(c.up_s),
+                          reinterpret_cast<const uint8_t*>(c.down_s), reinterpret_cast<const uint8_t*>(c.x_scale)};
+    return fused_moe_impl(c.x, c.gate, c.up, c.down, c.rw, c.idx, c.out, c.T, c.H, c.I, c.E, c.k, c.act, c.moe_type,
+                          c.dtype, nullptr, 0, true, !c.accumulate, s, nullptr, false, &mx);
 }
 
 }  // namespace cm
