@@ -392,8 +392,12 @@ static int dec_cap() { return 2 * 8 * std::max(cus_per_xcd(), 32); }
 // the decode kernels against 115 / 126 / 134 / 149 us; Qwen3 T=128 (256
 // pairs) 102 against 115 us.
 constexpr long long kDecDefaultPairs = 256;
-// MXFP4 weights: the same
-constexpr long long kMxDecPairs = 256;
+// MXFP4 weights: the decode kernels up to kMxDecPairs (steps, decode against
+// 32-row kernel: Qwen3 T=64 / 128 42 / 73 against 46 / 63 us, Qwen3-30B-A3B T=16 /
+// 32 73 / 118 against 80 / 107, H 768 I 2048 E 8 k 2 T=64 / 128 18 / 26 against 28 /
+// 27); most bytes for the 32-row kernel beyond 32 rows per touched expert.
+constexpr long long kMxDecPairs = 128;
+constexpr long long kMxRows32StreamBytes = 192LL << 20;
 // 16-bit prefill batches: rows per touched expert up to which nearly every
 // expert's rows fit one extended 128-row tile (160 rows: two standard
 // deviations of uniform routing above), and from which a 256-row tile often
@@ -511,8 +515,25 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
             return set_error(CANDLE_MOE_ERR_UNSUPPORTED,
                              "fused_moe_mxfp4: needs f16 or bf16, hidden_dim and intermediate_dim multiples of 32 and "
                              "16-byte aligned tensors (got dtype %u, %d, %d)", dtype, H, I);
-        p.cfg = P <= 32 * touched ? kLdsRows32 : P <= kOneTileRows * touched ? kLds128 : kLds256w8;
-        if (P <= kMxDecPairs && dec_gemv_fits(p)) p.cfg = kDecGemv;
+        // Decode kernels up to kMxDecPairs; the 32-row kernel, which streams an
+        // expert's codes once per 32 rows, up to 32 rows per touched expert or
+        // while that stream stays within kMxRows32StreamBytes; then, as for 16-bit
+        // weights, 128-row tiles while an expert's rows fit one, 128x128 where
+        // they are few or the 256x256 tiles number less than the CUs (steps, 32-row / 128x128 / 128x256 / 256x256 tiles: Qwen3
+        // T=256 73 / 79 / 127 / 97 us, T=500 115 / 90 / 145 / 123, T=1024 207 / 159
+        // / 150 / 157, T=2048 - / 294 / 283 / 223; Qwen3-30B-A3B T=1024 229 / 260 /
+        // 209 / 220, T=2048 369 / 322 / 281 / 289; H 768 I 2048 E 8 k 2 T=777 45 /
+        // 51 / 78 / 73, T=2000 73 / 71 / 90 / 87).
+        const long long stream = est_tiles(32) * (p.moe_type == kQwen3 ? 3LL : 2LL) * H * I * 17 / 32;
+        p.cfg = P <= kMxDecPairs && dec_gemv_fits(p) ? kDecGemv
+                : P <= 32 * touched || (P <= 256 * touched && stream <= kMxRows32StreamBytes) ? kLdsRows32
+                                                                                            : kLds256w8;
+        const int mode1 = p.moe_type == kQwen3 ? kGateUp : kFc1;
+        const long long dev_wgs = 8LL * std::max(cus_per_xcd(), 32);
+        if (p.cfg == kLds256w8 && P <= kOneTileRows * touched)
+            p.cfg = 2 * touched * cdiv(I, gemm_tile_cols(mode1, kLds128)) <= 3 * dev_wgs ? kLds128 : kLds128x256o2;
+        else if (p.cfg == kLds256w8 && H <= 1024 && est_tiles(256) * cdiv(I, gemm_tile_cols(mode1, kLds256w8)) < dev_wgs)
+            p.cfg = kLds128;
         if ((is_lds_cfg(g_tile_policy) && g_tile_policy != kW8Gemv) || (g_tile_policy == kDecGemv && dec_gemv_fits(p)))
             p.cfg = g_tile_policy;
     } else if (p.mfma && !policy) {
