@@ -12,12 +12,28 @@
 // counts as -infinity in the choice; logits of -infinity have score 0, also
 // where a row has no others (then every weight is 0).
 //
-// One wave per row; lane g owns the VPT experts from g * VPT on.
+// Two forms of a row:
+//
+//  exact: one wave per row, all scores and the choice in f64 (8 to 118 us for
+//    T = 32768 of 256 experts in 8 groups, bound by f64 exponentials and 64-bit
+//    exchanges). Every shape; and every row the fast form is not sure of.
+//  fast: LPR lanes per row, VPT experts each, scores in f32 within a known
+//    distance tau of the exact ones. A group's lanes are its own (padded), so
+//    its two best c meet in log2(lanes) exchanges, and its place among the groups
+//    is counted from their scores. The choice runs on 32-bit keys: c on a grid
+//    between the row's largest c and a bound the k + 1 best lie above, over the
+//    slot number: one v_max_u32 per exchange finds value and expert together.
+//    k + 2 rounds give the k best and the next two. Where two neighbours in that
+//    order (or a group at the border of the choice) are closer than 2 tau and the
+//    grid, and not an exact tie (equal logits and biases), or a value is not
+//    finite, the row goes the exact way: about one row in 500 of f32 logits. The
+//    k weights come from f64 exponentials of the chosen logits, one lane each.
 #include <limits.h>
 #include <math.h>
 
 #include "cm_common.hpp"
 #include "cm_internal.hpp"
+#include "cm_select.hpp"
 
 namespace cm {
 
@@ -25,11 +41,7 @@ namespace {
 
 constexpr int kRouteWaves = 4;
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-    return v;
-}
+__device__ __forceinline__ double wave_sum(double v) { return group_sum<64>(v); }
 
 // (value, index) of the best of the wave: the larger value, then the lower
 // index; index INT_MAX: none
@@ -43,17 +55,19 @@ __device__ __forceinline__ void wave_best(double& v, int& i) {
         i = take ? oi : i;
     }
 }
+// LDS written by some lanes of the wave is read by others (LDS operations of a
+// wave stay in order; this keeps the compiler's in order too)
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 
+// One row on one wave; buf: 64 * VPT doubles of this wave.
 template <int VPT, int DT>
-__global__ __launch_bounds__(64 * kRouteWaves) void route_k(RouteArgs a) {
+__device__ __forceinline__ void route_exact_row(const RouteArgs& a, long long row, double* buf) {
     typedef typename Elem<DT>::storage S;
-    __shared__ double s_buf[kRouteWaves][64 * VPT];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long row = (long long)blockIdx.x * kRouteWaves + wave;
-    const bool live = row < a.T;
-    const S* src = reinterpret_cast<const S*>(a.logits) + (live ? row : 0) * (long long)a.E;
-    double* buf = s_buf[wave];
-
+    const int lane = threadIdx.x & 63;
+    const S* src = reinterpret_cast<const S*>(a.logits) + row * (long long)a.E;
     double s[VPT], c[VPT];
     uint32_t alive = 0;
 #pragma unroll
@@ -92,7 +106,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_k(RouteArgs a) {
         const int per = a.E / a.groups;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) buf[lane * VPT + j] = c[j];
-        __syncthreads();
+        wave_lds_fence();
         double b1 = -(double)INFINITY, b2 = -(double)INFINITY;
         if (lane < a.groups) {
             for (int q = 0; q < per; ++q) {
@@ -115,7 +129,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_k(RouteArgs a) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
             if (!((keep >> ((lane * VPT + j) / per)) & 1ull)) alive &= ~(1u << j);
-        __syncthreads();
+        wave_lds_fence();
     }
 
     double total = 0.0;
@@ -142,37 +156,341 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_k(RouteArgs a) {
         total += w;
         if (lane == 0) {
             buf[q] = w;
-            if (live) a.idx[row * a.k + q] = (uint32_t)i;
+            a.idx[row * a.k + q] = (uint32_t)i;
         }
     }
-    __syncthreads();
-    if (!live) return;
+    wave_lds_fence();
     for (int q = lane; q < a.k; q += 64) {
         double w = buf[q];
         if (a.renorm) w = total == 0.0 ? 0.0 : w / total;
         a.w[row * a.k + q] = (float)(w * (double)a.scale);
         a.ei[row * a.k + q] = (uint32_t)((long long)q * a.T + row);
     }
+    wave_lds_fence();
+}
+
+template <int VPT, int DT>
+__global__ __launch_bounds__(64 * kRouteWaves) void route_exact_k(RouteArgs a) {
+    __shared__ double s_buf[kRouteWaves][64 * VPT];
+    const int wave = threadIdx.x >> 6;
+    const long long row = (long long)blockIdx.x * kRouteWaves + wave;
+    if (row < a.T) route_exact_row<VPT, DT>(a, row, s_buf[wave]);
+}
+
+// Sorted descending by Batcher's odd-even merges.
+template <int N>
+__device__ __forceinline__ void sort_desc(uint32_t* k) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+                        const uint32_t x = k[i + j], y = k[i + j + q];
+                        k[i + j] = max(x, y);
+                        k[i + j + q] = min(x, y);
+                    }
+}
+
+// v of the lane's partner over a step of 2M lanes, in f32 (both values to both lanes)
+template <int M>
+__device__ __forceinline__ void pair_f32(float v, float& x, float& y) {
+    uint32_t a, b;
+    lane_pair<M>(__float_as_uint(v), a, b);
+    x = __uint_as_float(a);
+    y = __uint_as_float(b);
+}
+// (b1, b2): the two largest of a group of lanes
+template <int M>
+__device__ __forceinline__ void top2_step(float& b1, float& b2) {
+    float p1, q1, p2, q2;
+    pair_f32<M>(b1, p1, q1);
+    pair_f32<M>(b2, p2, q2);
+    b1 = fmaxf(p1, q1);
+    b2 = fmaxf(fminf(p1, q1), fmaxf(p2, q2));
+}
+
+// lanes_log2: lanes of a group (all LPR with one group); cells: experts of a
+// group; vec: whole lanes of VPT values, 16-byte (or 8-byte) aligned; many: the
+// chosen groups have at least k + 1 lanes with experts.
+struct RouteFast {
+    int lanes_log2, cells, vec, many;
+};
+
+template <int LPR, int VPT, int DT>
+__global__ __launch_bounds__(64 * kRouteWaves) void route_fast_k(RouteArgs a, RouteFast f) {
+    typedef typename Elem<DT>::storage S;
+    constexpr int RPW = 64 / LPR, SLOTS = LPR * VPT, VS = SLOTS > 64 ? SLOTS / 64 : 1;
+    constexpr int IB = SLOTS == 64 ? 6 : SLOTS == 128 ? 7 : SLOTS == 256 ? 8 : SLOTS == 512 ? 9 : 10;
+    constexpr int QB = 32 - IB;
+    static_assert((1 << IB) == SLOTS, "slot bits");
+    __shared__ double s_buf[kRouteWaves][64 * VS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int sub = lane % LPR;
+    const long long row0 = ((long long)blockIdx.x * kRouteWaves + wave) * RPW;
+    if (row0 >= a.T) return;
+    const long long row = min(row0 + lane / LPR, (long long)a.T - 1);
+    const bool live = row0 + lane / LPR < a.T;
+    const int grp = sub >> f.lanes_log2;
+    const int cell = (sub - (grp << f.lanes_log2)) * VPT;  // first expert of this lane in its group
+    const int groups = a.topk_groups < a.groups ? a.groups : 1;
+    const int nval = grp < groups ? max(0, min(f.cells - cell, VPT)) : 0;
+    const int e0 = grp * f.cells + cell;
+    const S* src = reinterpret_cast<const S*>(a.logits) + row * (long long)a.E;
+
+    // scores and what the choice goes by; nothing: -infinity
+    float l[VPT], c[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) l[j] = 0.f;
+    if (f.vec) {
+        constexpr int BYTES = VPT * (int)sizeof(S);
+        if (nval) {
+            if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+                for (int v = 0; v < BYTES / 16; ++v) {
+                    const u32x4 q = reinterpret_cast<const u32x4*>(src + e0)[v];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        if constexpr (DT == kF32) {
+                            l[(4 * v + d) % VPT] = __uint_as_float(q[d]);
+                        } else {
+                            l[(8 * v + 2 * d) % VPT] = Elem<DT>::to_f32((uint16_t)(q[d] & 0xffffu));
+                            l[(8 * v + 2 * d + 1) % VPT] = Elem<DT>::to_f32((uint16_t)(q[d] >> 16));
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) l[j] = Elem<DT>::to_f32(src[e0 + j]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+            if (j < nval) l[j] = Elem<DT>::to_f32(src[e0 + j]);
+    }
+    float m = 0.f, tau = 3.5e-7f;
+    double total = 1.0;
+    if (a.score == kRouteSoftmax) {
+        m = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+            if (j < nval) m = fmaxf(m, l[j]);
+        m = group_max<LPR>(m);
+        float part[VPT];
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            c[j] = j < nval ? exp_f32_fast(l[j] - m) : 0.f;
+            part[j] = c[j];
+        }
+#pragma unroll
+        for (int q = VPT / 2; q >= 1; q /= 2)
+#pragma unroll
+            for (int j = 0; j < q; ++j) part[j] += part[j + q];
+        total = group_sum<LPR>((double)part[0]);
+        const float inv = (float)(1.0 / total);
+        tau = 7e-7f * inv;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) c[j] *= inv;
+    } else {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const float t = exp_f32_fast(-fabsf(l[j]));
+            c[j] = (l[j] < 0.f ? t : 1.f) * __builtin_amdgcn_rcpf(1.f + t);
+            c[j] = l[j] == l[j] ? c[j] : l[j];
+        }
+    }
+    if (a.bias) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j)
+            if (j < nval) c[j] += a.bias[e0 + j];
+    }
+    bool unsure = false;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        unsure |= j < nval && !__builtin_isfinite(c[j]);
+        c[j] = j < nval ? c[j] : -INFINITY;
+    }
+
+    bool kept = nval > 0;
+    if (groups > 1) {
+        float b1 = -INFINITY, b2 = -INFINITY, most = 0.f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            b2 = fmaxf(b2, fminf(b1, c[j]));
+            b1 = fmaxf(b1, c[j]);
+        }
+        if (f.lanes_log2 > 0) top2_step<1>(b1, b2);
+        if (f.lanes_log2 > 1) top2_step<2>(b1, b2);
+        if (f.lanes_log2 > 2) top2_step<4>(b1, b2);
+        if (f.lanes_log2 > 3) top2_step<8>(b1, b2);
+        if (f.lanes_log2 > 4) top2_step<16>(b1, b2);
+        const float gs = a.group_top == 1 ? b1 : b1 + b2;
+        most = fmaxf(fabsf(b1), fabsf(b2));
+        // two scores, each within tau and the roundings of c and the sum
+        const float far = 5.f * (tau + 1.2e-7f * (grp < groups ? most : 0.f));
+        const int base = lane - sub;
+        int above = 0, level = 0;
+        for (int q = 0; q < groups; ++q) {
+            const float v = __shfl(gs, base + (q << f.lanes_log2));
+            above += v > gs + far;
+            level += v >= gs - far;  // (itself among them)
+        }
+        kept = kept && level <= a.topk_groups;
+        unsure |= nval > 0 && level > a.topk_groups && above < a.topk_groups;
+    }
+
+    // the grid: [lo, hi] of what can be among the k + 1 best
+    float top = -INFINITY, low = INFINITY;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        top = fmaxf(top, c[j]);
+        if (j < nval) low = fminf(low, c[j]);
+    }
+    const float hi = group_max<LPR>(kept ? top : -INFINITY);
+    // (every one of `many` lanes holds a value >= the least of their largest)
+    const float lo = -group_max<LPR>(kept ? -(f.many ? top : low) : -INFINITY);
+    const float span = hi - lo;
+    const float unit = span > 0.f ? (float)((1u << QB) - 8u) / span : 0.f;
+    tau += 1.2e-7f * fmaxf(fabsf(hi), fabsf(lo));
+    // (f32 holds 24 bits of a grid of more)
+    const uint32_t apart = (uint32_t)fminf(2.f * tau * unit, 1e9f) + (16u << (QB > 24 ? QB - 24 : 0));
+    uint32_t key[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const uint32_t q = 1u + (uint32_t)fmaxf((c[j] - lo) * unit, 0.f);
+        key[j] = kept && j < nval ? (min(q, (1u << QB) - 1u) << IB) | (uint32_t)(SLOTS - 1 - (sub * VPT + j)) : 0u;
+    }
+    constexpr int NL = VPT > 8 ? VPT / 8 : 1, LEN = VPT / NL;  // sorted lists per lane
+#pragma unroll
+    for (int n = 0; n < NL; ++n) sort_desc<LEN>(key + n * LEN);
+    uint32_t mine = 0;  // lane r of the row: the key of place r
+    for (int r = 0; r <= a.k + 1; ++r) {
+        uint32_t h = key[0];
+        if constexpr (NL == 2) h = max(h, key[LEN]);
+        const uint32_t best = group_key32_max<LPR>(h);
+        mine = sub == r ? best : mine;
+#pragma unroll
+        for (int n = 0; n < NL; ++n) {
+            const uint64_t pop = __ballot(key[n * LEN] == best);
+#pragma unroll
+            for (int q = 0; q < LEN; ++q)
+                key[n * LEN + q] = key_take32(key[n * LEN + q], q + 1 < LEN ? key[n * LEN + (q + 1) % LEN] : 0u, pop);
+        }
+    }
+
+    // the chosen, one lane each; the distance to the next place
+    const int slot = SLOTS - 1 - (int)(mine & (SLOTS - 1));
+    const int sg = (slot / VPT) >> f.lanes_log2;
+    const int e = sg * f.cells + slot - (sg << f.lanes_log2) * VPT;
+    const bool has = sub <= a.k + 1 && mine != 0u;
+    const float le = has ? Elem<DT>::to_f32(src[e]) : 0.f;
+    const float be = has && a.bias ? a.bias[e] : 0.f;
+    const int next = min(lane + 1, 63);
+    const uint32_t nk = __shfl(mine, next);
+    const float nl = __shfl(le, next), nb = __shfl(be, next);
+    const bool near = nk != 0u && (mine >> IB) - (nk >> IB) <= apart;
+    const bool tie = le == nl && be == nb;
+    // (place k as far as k - 1 from the next where the two are a tie)
+    const int tied = __shfl_up((int)tie, 1);
+    unsure |= sub < a.k && (mine == 0u || (near && !tie));
+    unsure |= sub == a.k && mine != 0u && tied && near;
+    double w = 0.0;
+    if (sub < a.k) {
+        if (a.score == kRouteSoftmax) {
+            w = le == -INFINITY ? 0.0 : exp((double)le - (double)m);
+            if (!a.renorm) w /= total;
+        } else {
+            w = 1.0 / (1.0 + exp(-(double)le));
+        }
+    }
+    if (a.renorm) {
+        const double sum = group_sum<LPR>(w);
+        w = sum == 0.0 ? 0.0 : w / sum;
+    }
+    uint64_t redo = __ballot(unsure && live);
+    const uint64_t own = (LPR == 64 ? ~0ull : ((1ull << (LPR % 64)) - 1ull) << (lane - sub));
+    if (live && sub < a.k && !(redo & own)) {
+        const long long at = row * a.k + sub;
+        a.w[at] = (float)(w * (double)a.scale);
+        a.idx[at] = (uint32_t)e;
+        a.ei[at] = (uint32_t)((long long)sub * a.T + row);
+    }
+    while (redo) {
+        const int r = __builtin_ctzll(redo) / LPR;
+        route_exact_row<VS, DT>(a, row0 + r, s_buf[wave]);
+        redo &= ~(LPR == 64 ? ~0ull : ((1ull << (LPR % 64)) - 1ull) << (r * LPR));
+    }
 }
 
 template <int VPT>
-hipError_t launch_vpt(const RouteArgs& a, hipStream_t stream) {
+hipError_t launch_exact(const RouteArgs& a, hipStream_t stream) {
     const dim3 grid((unsigned)((a.T + kRouteWaves - 1) / kRouteWaves)), block(64 * kRouteWaves);
-    if (a.dtype == kF32) hipLaunchKernelGGL((route_k<VPT, kF32>), grid, block, 0, stream, a);
-    else if (a.dtype == kBF16) hipLaunchKernelGGL((route_k<VPT, kBF16>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((route_k<VPT, kF16>), grid, block, 0, stream, a);
+    if (a.dtype == kF32) hipLaunchKernelGGL((route_exact_k<VPT, kF32>), grid, block, 0, stream, a);
+    else if (a.dtype == kBF16) hipLaunchKernelGGL((route_exact_k<VPT, kBF16>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((route_exact_k<VPT, kF16>), grid, block, 0, stream, a);
     return hipGetLastError();
 }
+
+int next_pow2(int n) {
+    int p = 1;
+    while (p < n) p *= 2;
+    return p;
+}
+
+// f for LPR lanes of VPT experts, if the row fits them (a place per lane for the
+// k best and the next two).
+template <int LPR, int VPT>
+bool fits(const RouteArgs& a, RouteFast& f) {
+    const int groups = a.topk_groups < a.groups ? a.groups : 1;
+    f.cells = a.E / groups;
+    const int full = (f.cells + VPT - 1) / VPT;  // lanes with experts in a group
+    const int lanes = groups == 1 ? LPR : next_pow2(full);
+    if (full > lanes || next_pow2(groups) * lanes > LPR || a.k + 2 > LPR) return false;
+    f.lanes_log2 = __builtin_ctz(lanes);
+    f.many = (groups == 1 ? 1 : a.topk_groups) * full >= a.k + 1;
+    const int es = a.dtype == kF32 ? 4 : 2;
+    f.vec = f.cells % VPT == 0 && VPT * es % 16 == 0 && (long long)a.E * es % 16 == 0 &&
+            ((uintptr_t)a.logits & 15) == 0;
+    return true;
+}
+
+template <int LPR, int VPT>
+bool launch_fast(const RouteArgs& a, hipStream_t stream, hipError_t& e) {
+    RouteFast f;
+    if (!fits<LPR, VPT>(a, f)) return false;
+    const int rows = kRouteWaves * (64 / LPR);
+    const dim3 grid((unsigned)(((long long)a.T + rows - 1) / rows)), block(64 * kRouteWaves);
+    if (a.dtype == kF32) hipLaunchKernelGGL((route_fast_k<LPR, VPT, kF32>), grid, block, 0, stream, a, f);
+    else if (a.dtype == kBF16) hipLaunchKernelGGL((route_fast_k<LPR, VPT, kBF16>), grid, block, 0, stream, a, f);
+    else hipLaunchKernelGGL((route_fast_k<LPR, VPT, kF16>), grid, block, 0, stream, a, f);
+    e = hipGetLastError();
+    return true;
+}
+
+// Rows a launch needs before fewer lanes per row pay: with fewer the device is
+// not full either way and the shorter chains of 64 lanes are ahead.
+constexpr int kRouteManyRows = 2048;
 
 }  // namespace
 
 hipError_t launch_route(const RouteArgs& a, hipStream_t stream) {
     if (a.T <= 0) return hipSuccess;
-    if (a.E <= 64) return launch_vpt<1>(a, stream);
-    if (a.E <= 128) return launch_vpt<2>(a, stream);
-    if (a.E <= 256) return launch_vpt<4>(a, stream);
-    if (a.E <= 512) return launch_vpt<8>(a, stream);
-    return launch_vpt<16>(a, stream);
+    hipError_t e;
+    if (a.T >= kRouteManyRows &&
+        (launch_fast<16, 4>(a, stream, e) || launch_fast<16, 8>(a, stream, e) || launch_fast<32, 8>(a, stream, e)))
+        return e;
+    if (launch_fast<64, 2>(a, stream, e) || launch_fast<64, 4>(a, stream, e) || launch_fast<64, 8>(a, stream, e) ||
+        launch_fast<64, 16>(a, stream, e))
+        return e;
+    if (a.E <= 64) return launch_exact<1>(a, stream);
+    if (a.E <= 128) return launch_exact<2>(a, stream);
+    if (a.E <= 256) return launch_exact<4>(a, stream);
+    if (a.E <= 512) return launch_exact<8>(a, stream);
+    return launch_exact<16>(a, stream);
 }
 
 }  // namespace cm
