@@ -45,15 +45,25 @@ __device__ __forceinline__ double wave_sum(double v) { return group_sum<64>(v); 
 
 // (value, index) of the best of the wave: the larger value, then the lower
 // index; index INT_MAX: none
+template <int M>
+__device__ __forceinline__ void best_step(double& v, int& i) {
+    const uint64_t u = __double_as_longlong(v);
+    uint32_t al, bl, ah, bh, ai, bi;
+    lane_pair<M>((uint32_t)u, al, bl);
+    lane_pair<M>((uint32_t)(u >> 32), ah, bh);
+    lane_pair<M>((uint32_t)i, ai, bi);
+    const double x = __longlong_as_double(((uint64_t)ah << 32) | al), y = __longlong_as_double(((uint64_t)bh << 32) | bl);
+    const bool take = (int)bi != INT_MAX && ((int)ai == INT_MAX || y > x || (y == x && (int)bi < (int)ai));
+    v = take ? y : x;
+    i = (int)(take ? bi : ai);
+}
 __device__ __forceinline__ void wave_best(double& v, int& i) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const double ov = __shfl_xor(v, m);
-        const int oi = __shfl_xor(i, m);
-        const bool take = oi != INT_MAX && (i == INT_MAX || ov > v || (ov == v && oi < i));
-        v = take ? ov : v;
-        i = take ? oi : i;
-    }
+    best_step<1>(v, i);
+    best_step<2>(v, i);
+    best_step<4>(v, i);
+    best_step<8>(v, i);
+    best_step<16>(v, i);
+    best_step<32>(v, i);
 }
 // LDS written by some lanes of the wave is read by others (LDS operations of a
 // wave stay in order; this keeps the compiler's in order too)
@@ -214,13 +224,14 @@ __device__ __forceinline__ void top2_step(float& b1, float& b2) {
 }
 
 // lanes_log2: lanes of a group (all LPR with one group); cells: experts of a
-// group; vec: whole lanes of VPT values, 16-byte (or 8-byte) aligned; many: the
-// chosen groups have at least k + 1 lanes with experts.
+// group; many: the chosen groups have at least k + 2 lanes with experts.
 struct RouteFast {
-    int lanes_log2, cells, vec, many;
+    int lanes_log2, cells, many;
 };
 
-template <int LPR, int VPT, int DT>
+// WHOLE: every lane holds VPT experts or none, and logits and biases are read 16
+// bytes at a time.
+template <int LPR, int VPT, int DT, bool WHOLE>
 __global__ __launch_bounds__(64 * kRouteWaves) void route_fast_k(RouteArgs a, RouteFast f) {
     typedef typename Elem<DT>::storage S;
     constexpr int RPW = 64 / LPR, SLOTS = LPR * VPT, VS = SLOTS > 64 ? SLOTS / 64 : 1;
@@ -240,50 +251,59 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_fast_k(RouteArgs a, Ro
     const int nval = grp < groups ? max(0, min(f.cells - cell, VPT)) : 0;
     const int e0 = grp * f.cells + cell;
     const S* src = reinterpret_cast<const S*>(a.logits) + row * (long long)a.E;
+    auto ours = [&](int j) { return WHOLE ? nval > 0 : j < nval; };
 
-    // scores and what the choice goes by; nothing: -infinity
-    float l[VPT], c[VPT];
+    // scores and what the choice goes by
+    float l[VPT], c[VPT], b[VPT];
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) l[j] = 0.f;
-    if (f.vec) {
-        constexpr int BYTES = VPT * (int)sizeof(S);
+    for (int j = 0; j < VPT; ++j) l[j] = b[j] = 0.f;
+    if constexpr (WHOLE) {
         if (nval) {
-            if constexpr (BYTES % 16 == 0) {
 #pragma unroll
-                for (int v = 0; v < BYTES / 16; ++v) {
-                    const u32x4 q = reinterpret_cast<const u32x4*>(src + e0)[v];
+            for (int v = 0; v < VPT * (int)sizeof(S) / 16; ++v) {
+                const u32x4 q = reinterpret_cast<const u32x4*>(src + e0)[v];
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        if constexpr (DT == kF32) {
-                            l[(4 * v + d) % VPT] = __uint_as_float(q[d]);
-                        } else {
-                            l[(8 * v + 2 * d) % VPT] = Elem<DT>::to_f32((uint16_t)(q[d] & 0xffffu));
-                            l[(8 * v + 2 * d + 1) % VPT] = Elem<DT>::to_f32((uint16_t)(q[d] >> 16));
-                        }
+                for (int d = 0; d < 4; ++d) {
+                    if constexpr (DT == kF32) {
+                        l[(4 * v + d) % VPT] = __uint_as_float(q[d]);
+                    } else {
+                        l[(8 * v + 2 * d) % VPT] = Elem<DT>::to_f32((uint16_t)(q[d] & 0xffffu));
+                        l[(8 * v + 2 * d + 1) % VPT] = Elem<DT>::to_f32((uint16_t)(q[d] >> 16));
                     }
                 }
-            } else {
+            }
+            if (a.bias) {
 #pragma unroll
-                for (int j = 0; j < VPT; ++j) l[j] = Elem<DT>::to_f32(src[e0 + j]);
+                for (int v = 0; v < VPT / 4; ++v) {
+                    const f32x4 q = reinterpret_cast<const f32x4*>(a.bias + e0)[v];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) b[(4 * v + d) % VPT] = q[d];
+                }
             }
         }
     } else {
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
-            if (j < nval) l[j] = Elem<DT>::to_f32(src[e0 + j]);
+            if (j < nval) {
+                l[j] = Elem<DT>::to_f32(src[e0 + j]);
+                if (a.bias) b[j] = a.bias[e0 + j];
+            }
     }
+    // 2^(x log2 e) by v_exp_f32: the product's rounding is |x| 2^-24 of the value,
+    // at most 0.23 * 2^-24 of a sigmoid (s (1 - s) |x|) and 0.37 * 2^-24 of the
+    // largest exponential of a softmax (|x| e^-|x|)
+    constexpr float kLog2e = 1.44269504088896341f;
     float m = 0.f, tau = 3.5e-7f;
     double total = 1.0;
     if (a.score == kRouteSoftmax) {
         m = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < VPT; ++j)
-            if (j < nval) m = fmaxf(m, l[j]);
+        for (int j = 0; j < VPT; ++j) m = ours(j) ? fmaxf(m, l[j]) : m;
         m = group_max<LPR>(m);
         float part[VPT];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            c[j] = j < nval ? exp_f32_fast(l[j] - m) : 0.f;
+            c[j] = ours(j) ? __builtin_amdgcn_exp2f((l[j] - m) * kLog2e) : 0.f;
             part[j] = c[j];
         }
 #pragma unroll
@@ -291,33 +311,28 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_fast_k(RouteArgs a, Ro
 #pragma unroll
             for (int j = 0; j < q; ++j) part[j] += part[j + q];
         total = group_sum<LPR>((double)part[0]);
-        const float inv = (float)(1.0 / total);
-        tau = 7e-7f * inv;
+        const float inv = __builtin_amdgcn_rcpf((float)total);
+        tau = 9e-7f * inv;
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) c[j] *= inv;
+        for (int j = 0; j < VPT; ++j) c[j] = fmaf(c[j], inv, b[j]);
     } else {
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const float t = exp_f32_fast(-fabsf(l[j]));
-            c[j] = (l[j] < 0.f ? t : 1.f) * __builtin_amdgcn_rcpf(1.f + t);
-            c[j] = l[j] == l[j] ? c[j] : l[j];
+            const float t = __builtin_amdgcn_exp2f(fabsf(l[j]) * -kLog2e);
+            c[j] = fmaf(l[j] < 0.f ? t : 1.f, __builtin_amdgcn_rcpf(1.f + t), b[j]);  // (a NaN through t)
         }
     }
-    if (a.bias) {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j)
-            if (j < nval) c[j] += a.bias[e0 + j];
-    }
-    bool unsure = false;
+    float zero = 0.f;  // NaN where a value is not finite
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        unsure |= j < nval && !__builtin_isfinite(c[j]);
-        c[j] = j < nval ? c[j] : -INFINITY;
+        zero = ours(j) ? fmaf(c[j], 0.f, zero) : zero;
+        c[j] = ours(j) ? c[j] : -INFINITY;
     }
+    bool unsure = !(zero == 0.f);
 
     bool kept = nval > 0;
     if (groups > 1) {
-        float b1 = -INFINITY, b2 = -INFINITY, most = 0.f;
+        float b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             b2 = fmaxf(b2, fminf(b1, c[j]));
@@ -329,8 +344,8 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_fast_k(RouteArgs a, Ro
         if (f.lanes_log2 > 3) top2_step<8>(b1, b2);
         if (f.lanes_log2 > 4) top2_step<16>(b1, b2);
         const float gs = a.group_top == 1 ? b1 : b1 + b2;
-        most = fmaxf(fabsf(b1), fabsf(b2));
-        // two scores, each within tau and the roundings of c and the sum
+        // two scores of one or two c, each within tau and its rounding, and the sum's
+        const float most = a.group_top == 1 ? fabsf(b1) : fmaxf(fabsf(b1), fabsf(b2));
         const float far = 5.f * (tau + 1.2e-7f * (grp < groups ? most : 0.f));
         const int base = lane - sub;
         int above = 0, level = 0;
@@ -339,30 +354,34 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_fast_k(RouteArgs a, Ro
             above += v > gs + far;
             level += v >= gs - far;  // (itself among them)
         }
-        kept = kept && level <= a.topk_groups;
         unsure |= nval > 0 && level > a.topk_groups && above < a.topk_groups;
+        kept = kept && level <= a.topk_groups;
     }
 
-    // the grid: [lo, hi] of what can be among the k + 1 best
+    // the grid: [lo, hi] of what can be among the k + 2 best
     float top = -INFINITY, low = INFINITY;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-        top = fmaxf(top, c[j]);
-        if (j < nval) low = fminf(low, c[j]);
+    for (int j = 0; j < VPT; ++j) top = fmaxf(top, c[j]);
+    low = top;
+    if (!f.many) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) low = ours(j) ? fminf(low, c[j]) : low;
     }
     const float hi = group_max<LPR>(kept ? top : -INFINITY);
-    // (every one of `many` lanes holds a value >= the least of their largest)
-    const float lo = -group_max<LPR>(kept ? -(f.many ? top : low) : -INFINITY);
+    // (with many lanes each holds a value >= the least of their largest)
+    const float lo = -group_max<LPR>(kept ? -low : -INFINITY);
     const float span = hi - lo;
-    const float unit = span > 0.f ? (float)((1u << QB) - 8u) / span : 0.f;
-    tau += 1.2e-7f * fmaxf(fabsf(hi), fabsf(lo));
+    const float unit = span > 0.f ? (float)((1u << QB) - 16u) * __builtin_amdgcn_rcpf(span) : 0.f;
+    const float first = fmaf(-lo, unit, 4.f);
+    tau += 3.6e-7f * fmaxf(fabsf(hi), fabsf(lo));  // roundings of c, of first and of the product
     // (f32 holds 24 bits of a grid of more)
     const uint32_t apart = (uint32_t)fminf(2.f * tau * unit, 1e9f) + (16u << (QB > 24 ? QB - 24 : 0));
     uint32_t key[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        const uint32_t q = 1u + (uint32_t)fmaxf((c[j] - lo) * unit, 0.f);
-        key[j] = kept && j < nval ? (min(q, (1u << QB) - 1u) << IB) | (uint32_t)(SLOTS - 1 - (sub * VPT + j)) : 0u;
+        // (the conversion takes what is below the grid, and a NaN, to 0)
+        const uint32_t q = (uint32_t)__builtin_amdgcn_fmed3f(fmaf(c[j], unit, first), 1.f, (float)((1u << QB) - 1u));
+        key[j] = kept && ours(j) ? (q << IB) | (uint32_t)(SLOTS - 1 - (sub * VPT + j)) : 0u;
     }
     constexpr int NL = VPT > 8 ? VPT / 8 : 1, LEN = VPT / NL;  // sorted lists per lane
 #pragma unroll
@@ -382,31 +401,52 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_fast_k(RouteArgs a, Ro
         }
     }
 
-    // the chosen, one lane each; the distance to the next place
+    // places 0 .. k + 1, one lane each, and their scores in 64 bits
     const int slot = SLOTS - 1 - (int)(mine & (SLOTS - 1));
     const int sg = (slot / VPT) >> f.lanes_log2;
-    const int e = sg * f.cells + slot - (sg << f.lanes_log2) * VPT;
     const bool has = sub <= a.k + 1 && mine != 0u;
-    const float le = has ? Elem<DT>::to_f32(src[e]) : 0.f;
-    const float be = has && a.bias ? a.bias[e] : 0.f;
-    const int next = min(lane + 1, 63);
-    const uint32_t nk = __shfl(mine, next);
-    const float nl = __shfl(le, next), nb = __shfl(be, next);
-    const bool near = nk != 0u && (mine >> IB) - (nk >> IB) <= apart;
-    const bool tie = le == nl && be == nb;
-    // (place k as far as k - 1 from the next where the two are a tie)
-    const int tied = __shfl_up((int)tie, 1);
-    unsure |= sub < a.k && (mine == 0u || (near && !tie));
-    unsure |= sub == a.k && mine != 0u && tied && near;
+    int e = has ? sg * f.cells + slot - (sg << f.lanes_log2) * VPT : INT_MAX;
+    const float le = has ? Elem<DT>::to_f32(src[e]) : -INFINITY;
+    const double be = has && a.bias ? (double)a.bias[e] : 0.0;
+    const bool soft = a.score == kRouteSoftmax;
     double w = 0.0;
-    if (sub < a.k) {
-        if (a.score == kRouteSoftmax) {
-            w = le == -INFINITY ? 0.0 : exp((double)le - (double)m);
-            if (!a.renorm) w /= total;
-        } else {
-            w = 1.0 / (1.0 + exp(-(double)le));
+    if (has) {
+        const double x = exp(soft ? (double)le - (double)m : -(double)le);
+        w = soft ? (le == -INFINITY ? 0.0 : x) : 1.0 / (1.0 + x);
+    }
+    // No other expert can be among the k best if place k + 1 is clear of place
+    // k - 1; the order of places 0 .. k goes by their exact c (those of a softmax
+    // with a bias would need the exact sum: those rows need clear places).
+    const uint32_t k1 = __shfl_down(mine, 1), k2 = __shfl_down(mine, 2);
+    unsure |= sub < a.k && mine == 0u;
+    unsure |= sub == a.k - 1 && k2 != 0u && (mine >> IB) - (k2 >> IB) <= apart;
+    if (soft && a.bias) {
+        const float nl = __shfl_down(le, 1);
+        const double nb = __shfl_down(be, 1);
+        unsure |= sub < a.k && k1 != 0u && (mine >> IB) - (k1 >> IB) <= apart && !(le == nl && be == nb);
+    } else {
+        const double ce = w + be;
+        const double nc = __shfl_down(ce, 1);
+        const int ne = __shfl_down(e, 1);
+        const bool wrong = sub < a.k && ne != INT_MAX && (nc > ce || (nc == ce && ne < e));
+        if (__any(wrong)) {
+            const int base = lane - sub;
+            int place = 0;
+            for (int q = 0; q <= a.k; ++q) {
+                const double vc = __shfl(ce, base + q);
+                const int ve = __shfl(e, base + q);
+                place += ve != INT_MAX && (vc > ce || (vc == ce && ve < e));
+            }
+            const int to = 4 * (sub <= a.k && e != INT_MAX ? base + place : lane);
+            const uint64_t u = __double_as_longlong(w);
+            e = __builtin_amdgcn_ds_permute(to, e);
+            const uint32_t wl = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)u);
+            const uint32_t wh = (uint32_t)__builtin_amdgcn_ds_permute(to, (int)(uint32_t)(u >> 32));
+            w = __longlong_as_double(((uint64_t)wh << 32) | wl);
         }
     }
+    w = sub < a.k ? w : 0.0;
+    if (soft && !a.renorm) w /= total;
     if (a.renorm) {
         const double sum = group_sum<LPR>(w);
         w = sum == 0.0 ? 0.0 : w / sum;
@@ -444,29 +484,41 @@ int next_pow2(int n) {
 // f for LPR lanes of VPT experts, if the row fits them (a place per lane for the
 // k best and the next two).
 template <int LPR, int VPT>
-bool fits(const RouteArgs& a, RouteFast& f) {
+bool fits(const RouteArgs& a, RouteFast& f, bool& whole) {
     const int groups = a.topk_groups < a.groups ? a.groups : 1;
     f.cells = a.E / groups;
     const int full = (f.cells + VPT - 1) / VPT;  // lanes with experts in a group
     const int lanes = groups == 1 ? LPR : next_pow2(full);
     if (full > lanes || next_pow2(groups) * lanes > LPR || a.k + 2 > LPR) return false;
     f.lanes_log2 = __builtin_ctz(lanes);
-    f.many = (groups == 1 ? 1 : a.topk_groups) * full >= a.k + 1;
+    f.many = (groups == 1 ? 1 : a.topk_groups) * full >= a.k + 2;
     const int es = a.dtype == kF32 ? 4 : 2;
-    f.vec = f.cells % VPT == 0 && VPT * es % 16 == 0 && (long long)a.E * es % 16 == 0 &&
-            ((uintptr_t)a.logits & 15) == 0;
+    whole = f.cells % VPT == 0 && VPT * es % 16 == 0 && (long long)a.E * es % 16 == 0 &&
+            (((uintptr_t)a.logits | (uintptr_t)a.bias) & 15) == 0;
     return true;
 }
 
+template <int LPR, int VPT, int DT>
+void launch_form(const RouteArgs& a, const RouteFast& f, bool whole, const dim3& grid, hipStream_t stream) {
+    const dim3 block(64 * kRouteWaves);
+    if constexpr (VPT * (DT == kF32 ? 4 : 2) % 16 == 0) {
+        if (whole) {
+            hipLaunchKernelGGL((route_fast_k<LPR, VPT, DT, true>), grid, block, 0, stream, a, f);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((route_fast_k<LPR, VPT, DT, false>), grid, block, 0, stream, a, f);
+}
 template <int LPR, int VPT>
 bool launch_fast(const RouteArgs& a, hipStream_t stream, hipError_t& e) {
     RouteFast f;
-    if (!fits<LPR, VPT>(a, f)) return false;
+    bool whole;
+    if (!fits<LPR, VPT>(a, f, whole)) return false;
     const int rows = kRouteWaves * (64 / LPR);
-    const dim3 grid((unsigned)(((long long)a.T + rows - 1) / rows)), block(64 * kRouteWaves);
-    if (a.dtype == kF32) hipLaunchKernelGGL((route_fast_k<LPR, VPT, kF32>), grid, block, 0, stream, a, f);
-    else if (a.dtype == kBF16) hipLaunchKernelGGL((route_fast_k<LPR, VPT, kBF16>), grid, block, 0, stream, a, f);
-    else hipLaunchKernelGGL((route_fast_k<LPR, VPT, kF16>), grid, block, 0, stream, a, f);
+    const dim3 grid((unsigned)(((long long)a.T + rows - 1) / rows));
+    if (a.dtype == kF32) launch_form<LPR, VPT, kF32>(a, f, whole, grid, stream);
+    else if (a.dtype == kBF16) launch_form<LPR, VPT, kBF16>(a, f, whole, grid, stream);
+    else launch_form<LPR, VPT, kF16>(a, f, whole, grid, stream);
     e = hipGetLastError();
     return true;
 }
@@ -481,7 +533,8 @@ hipError_t launch_route(const RouteArgs& a, hipStream_t stream) {
     if (a.T <= 0) return hipSuccess;
     hipError_t e;
     if (a.T >= kRouteManyRows &&
-        (launch_fast<16, 4>(a, stream, e) || launch_fast<16, 8>(a, stream, e) || launch_fast<32, 8>(a, stream, e)))
+        (launch_fast<16, 4>(a, stream, e) || launch_fast<16, 8>(a, stream, e) || launch_fast<16, 16>(a, stream, e) ||
+         launch_fast<32, 8>(a, stream, e) || launch_fast<32, 16>(a, stream, e)))
         return e;
     if (launch_fast<64, 2>(a, stream, e) || launch_fast<64, 4>(a, stream, e) || launch_fast<64, 8>(a, stream, e) ||
         launch_fast<64, 16>(a, stream, e))
