@@ -877,10 +877,10 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
         d.scale1 = f8->up_scale;
     }
     if (mx) {
-        d.w4 = 1;
         d.mx0 = mx->gate_s;
         d.mx1 = mx->up_s;
         d.xs = mx->x_s;
+        d.kc = mx_dec_chunk((int)std::min<long long>(p.P, p.T), p.H, mx->x_s ? 1 : 2);
     }
     const int es = p.dtype == kF32 ? 4 : 2;
     d.a_bytes = (long long)p.T * p.H * (mx && mx->x_s ? 1 : es);
@@ -888,14 +888,14 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     d.rows_max = (int)std::min<long long>(p.P, p.T);
     d.cap = dec_cap();
     d.ks_lim = p.dec_ks1;
-    const int most_cpl = mx && d.rows_max > 16 ? 6 : 8;  // (launch_cfg)
+    const int most_cpl = mx && d.rows_max > 16 ? 6 : 8;  // (launch_mx_dec)
     d.cpl = dec_cpl(d.max_groups, p.I, !nk, d.ks_lim, p.dtype == kF32, most_cpl);
     d.nblk = cdiv(p.I, 16 * d.cpl);
     const int mode1 = qwen3 ? kGateUp : kFc1;
     hipError_t e;
     {
         ProfScope ps(kSlotGemm1, s);
-        e = launch_dec_gemv(mode1, p.dtype, d, s);
+        e = mx ? launch_mx_dec(mode1, p.dtype, d, s) : launch_dec_gemv(mode1, p.dtype, d, s);
         if (e == hipSuccess && d.ks_lim > 1) {
             DecFinish f = {};
             f.part = part;
@@ -926,6 +926,7 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     if (mx) {
         d2.mx0 = qwen3 ? mx->down_s : mx->up_s;
         d2.mx1 = d2.xs = nullptr;
+        d2.kc = mx_dec_chunk(d.rows_max, p.I, 2);
     }
     d2.a_bytes = p.P * p.I * es;
     d2.ks_lim = p.dec_ks2;
@@ -938,7 +939,8 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     d2.nblk = cdiv(p.H, 16 * d2.cpl);
     {
         ProfScope ps(kSlotGemm2, s);
-        e = launch_dec_gemv(qwen3 ? kDownRows : kFc2Rows, p.dtype, d2, s);
+        e = mx ? launch_mx_dec(kDownRows, p.dtype, d2, s)
+               : launch_dec_gemv(qwen3 ? kDownRows : kFc2Rows, p.dtype, d2, s);
     }
     if (e != hipSuccess) return hip_fail(e, "fused_moe decode down GEMM");
     {

@@ -349,12 +349,18 @@ struct DecArgs {
     int w8;                   // fp8 e4m3 codes [E][N][K] (ldb = K) with f32 scales [E][N]
     const float* scale0;      // (w8) gate / fc1 column scales (kGateUp / kFc1 with ks == 1)
     const float* scale1;      // (w8) up column scales
-    int w4;                   // MXFP4 codes [E][N][K/2] (ldb = K), K a multiple of 32
-    const uint8_t* mx0;       // (w4) scale bytes [E][N][K/32] of B0
-    const uint8_t* mx1;       // (w4) and of B1
-    const uint8_t* xs;        // (w4, kGateUp / kFc1) A is MXFP8 codes: their scale bytes [T][K/32]
+    const uint8_t* mx0;       // launch_mx_dec: scale bytes [E][N][K/32] of B0 (codes [E][N][K/2])
+    const uint8_t* mx1;       // and of B1
+    const uint8_t* xs;        // (kGateUp / kFc1) A is MXFP8 codes: their scale bytes [T][K/32], else null
+    int kc;                   // k of a row staged in LDS at a time (mx_dec_chunk)
 };
 hipError_t launch_dec_gemv(int mode, int dtype, const DecArgs& a, hipStream_t stream);
+// Decode GEMMs over MXFP4 weights (moe_gemv_mx.hip): kGateUp, kFc1 (inter [P, N] by
+// pair in the dtype), kDownRows / kFc2Rows (f32 partials, one slice); ks_lim 1,
+// cpl 2, 3, 4, 6 or (rows_max <= 16) 8.
+constexpr int kMxDecLds = 144 * 1024;
+int mx_dec_chunk(int rows_max, int K, int row_bytes);
+hipError_t launch_mx_dec(int mode, int dtype, const DecArgs& a, hipStream_t stream);
 // Finishing the K slices of a decode GEMM (fixed slice order: deterministic),
 // ks = meta[0] (gate/up, fc1) or meta[1] (down, fc2), as the GEMM stored it.
 // kGateUp / kFc1 (nothing to do when ks == 1): inter[p] = dtype(act(s0 *

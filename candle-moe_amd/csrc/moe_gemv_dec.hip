@@ -42,40 +42,23 @@
 // the activation for gate/up / fc1, out[t] = dtype(sum_j w_{t,j} * ...) over
 // a token's k pairs in slot order for down / fc2. No workgroup reads what
 // another writes: the kernel boundaries order the launches.
-#include "cm_lds.hpp"
+#include "cm_dec.hpp"
 
 namespace cm {
 
 using namespace lds;
+using namespace dec;
 
 namespace {
-
-template <int DT>
-__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
-    if constexpr (DT == kBF16) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
-                                                       c, 0, 0, 0);
-    } else {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c,
-                                                      0, 0, 0);
-    }
-}
-
-// Weight formats of moe_dec_gemv beside the activation dtype
-enum DecWeights : int { kDecFp8 = 1, kDecMxfp4 = 2 };
 
 constexpr int kDvWaves = 4;  // waves per workgroup
 constexpr int kDvStep = 32;  // K per step (one MFMA deep)
 // steps in flight per wave: 4, or 2 for 6 or 8 columns per lane, so that a
 // wave stays within 256 registers and two workgroups share a CU; halved where
 // each column takes WCH = 2 chunks of 16 bytes per step (the same bytes in
-// flight). f32 (4 columns): twice the bytes per weight, so 2 steps. MXFP4: a step
-// is 128 k, whose rows take four loads each, so fewer with two row blocks.
-template <int CPL, int WCH = 1, bool F32 = false, bool W4 = false, int RB = 1>
-constexpr int dec_ring() {
-    if (W4) return CPL >= 6 || (RB == 2 && CPL > 2) ? 2 : CPL == 4 ? 3 : 4;
-    return F32 ? 2 : (CPL >= 6 ? 2 : 4) / WCH;
-}
+// flight). f32 (4 columns): twice the bytes per weight, so 2 steps.
+template <int CPL, int WCH = 1, bool F32 = false>
+constexpr int dec_ring() { return F32 ? 2 : (CPL >= 6 ? 2 : 4) / WCH; }
 
 // Operand j of a transposed 8 x CPL block: r[t] holds k-row t of CPL
 // consecutive columns (pairs of 16-bit values, low half first); the result
@@ -87,100 +70,6 @@ __device__ __forceinline__ u32x4 column_operand(const uint32_t (&r)[8][CPL / 2],
 #pragma unroll
     for (int q = 0; q < 4; ++q) o[q] = __builtin_amdgcn_perm(r[2 * q + 1][j >> 1], r[2 * q][j >> 1], sel);
     return o;
-}
-
-// The touched-expert bitmap (LDS; the expert ids are kept in s_idx, -1:
-// dropped) and this workgroup's item. With U touched experts and nblk column
-// blocks, K is split into ks = min(cap / (U * nblk), ks_lim) slices (at least
-// 1), so that the U * nblk * ks items fill one round of cap workgroups;
-// workgroup w takes item w: the u-th touched expert (u = w / (nblk * ks)), a
-// column block and a slice. [K,N] weights: the column blocks vary fastest,
-// so that workgroups running side by side read neighbouring runs of the same
-// k-rows; [N,K]: the slices, for neighbouring K runs of the same columns.
-// s_misc[0..3] = expert (-1: no item), column block, slice, ks. Workgroup 0
-// also stores ks to meta[slot] for the finishing launch.
-template <int NT, bool TRANS>
-__device__ __forceinline__ void dec_assign(const DecArgs& a, int slot, uint32_t* s_bm, int32_t* s_idx,
-                                           int* s_misc) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int nwords = (a.E + 31) >> 5;
-    for (int w = tid; w < nwords; w += NT) s_bm[w] = 0u;
-    __syncthreads();
-    for (int p = tid; p < a.P; p += NT) {
-        const uint32_t e = a.idx[p];
-        const bool ok = e < (uint32_t)a.E;
-        s_idx[p] = ok ? (int)e : -1;
-        if (ok) atomicOr(&s_bm[e >> 5], 1u << (e & 31));
-    }
-    __syncthreads();
-    // wave 0: touched experts U, the slices, the item and its expert (the
-    // u-th set bit; each lane two words: E <= 4096)
-    if (wave == 0) {
-        const uint32_t w0 = 2 * lane < nwords ? s_bm[2 * lane] : 0u;
-        const uint32_t w1 = 2 * lane + 1 < nwords ? s_bm[2 * lane + 1] : 0u;
-        const int c = __popc(w0) + __popc(w1);
-        int incl = c;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int v = __shfl_up(incl, off);
-            if (lane >= off) incl += v;
-        }
-        const int excl = incl - c;
-        const int U = __shfl(incl, 63);
-        const long long un = (long long)U * a.nblk;
-        const int ks = un > 0 ? (int)max(1LL, min((long long)a.cap / un, (long long)a.ks_lim)) : 1;
-        const long long w = blockIdx.x;
-        const int per_u = a.nblk * ks;
-        const int u = (int)(w / per_u);
-        const int r_u = (int)(w - (long long)u * per_u);
-        const int sl = TRANS ? r_u / a.nblk : r_u % ks;
-        const int cb = TRANS ? r_u - sl * a.nblk : r_u / ks;
-        if (lane == 0) {
-            s_misc[0] = -1;
-            s_misc[1] = cb;
-            s_misc[2] = sl;
-            s_misc[3] = ks;
-            if (blockIdx.x == 0) a.meta[slot] = ks;
-        }
-        __builtin_amdgcn_wave_barrier();
-        if (u < U && u >= excl && u < incl) {
-            int need = u - excl;  // set bits to skip in this lane's words
-            uint32_t wd = w0;
-            int base = 64 * lane;
-            if (need >= __popc(w0)) {
-                need -= __popc(w0);
-                wd = w1;
-                base += 32;
-            }
-            for (int q = 0; q < need; ++q) wd &= wd - 1u;  // drop the lowest set bits
-            s_misc[0] = base + __builtin_ctz(wd);
-        }
-    }
-    __syncthreads();
-}
-
-// Expert e's pairs, ascending (a stable compaction of s_idx over NT-pair
-// chunks), into s_rows; returns their number.
-template <int NT>
-__device__ __forceinline__ int dec_rows(const DecArgs& a, int e, const int32_t* s_idx, int32_t* s_rows,
-                                        int* s_misc) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int run = 0;
-    for (int p0 = 0; p0 < a.P; p0 += NT) {
-        const int p = p0 + tid;
-        const bool hit = p < a.P && s_idx[p] == e;
-        const uint64_t m = __ballot(hit);
-        if (lane == 0) s_misc[8 + wave] = __popcll(m);
-        __syncthreads();
-        int before = run;
-        for (int w = 0; w < wave; ++w) before += s_misc[8 + w];
-        int total = run;
-        for (int w = 0; w < NT / 64; ++w) total += s_misc[8 + w];
-        if (hit) s_rows[before + __popcll(m & ((1ull << lane) - 1ull))] = p;
-        run = total;
-        __syncthreads();
-    }
-    return run;
 }
 
 // Finishing the K slices (fixed slice and slot order). Up to KSM slices and
@@ -293,14 +182,13 @@ __device__ __forceinline__ void finish_token4(const DecFinish& f, int ks, long l
     }
 }
 
-template <int DT, int MODE, int RB, int CPL, bool PK, int WQ, bool X8 = false>
+template <int DT, int MODE, int RB, int CPL, bool PK, bool W8>
 __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     constexpr bool DUAL = (MODE == kGateUp);
     constexpr bool GATHER = (MODE == kGateUp || MODE == kFc1);
     // [K,N] weights (the API layout but Nomic's fc2); [N,K]: fc2, every GEMM
-    // on pre-packed weights (PK) and on fp8 (W8) or MXFP4 (W4) codes
-    constexpr bool W8 = WQ == kDecFp8, W4 = WQ == kDecMxfp4;
-    constexpr bool TRANS = (MODE != kFc2Rows) && !PK && !W8 && !W4;
+    // on pre-packed weights (PK) and on fp8 codes (W8)
+    constexpr bool TRANS = (MODE != kFc2Rows) && !PK && !W8;
     // W8: OCP fp8 e4m3 codes [E][N][K] (one byte per weight) with per-column
     // f32 scales. A step is 128 k: a lane's two 16-byte loads hold
     // k0 + 32g .. +31 of its column, the operands of four MFMAs (converted
@@ -319,20 +207,14 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     // form (whose v_perm transpose the pairwise conversion replaces); [N,K]:
     // two 16-byte chunks of 4 k, 128 contiguous bytes per column and step.
     constexpr bool F32 = DT == kF32;
-    static_assert(!F32 || (!W8 && !W4 && !PK && CPL == 4), "f32: API layout, 4 columns per lane");
-    // W4: MXFP4 codes [E][N][K/2]; a lane's 16-byte chunk holds the 32 k of one
-    // scale (scales [E][N][K/32], a byte load beside it), which the gfx950 scaled
-    // conversion applies while it turns the codes into DT operands, exactly.
-    // X8: the rows are MXFP8 codes with a scale byte per 32 k (xs), converted the
-    // same way.
-    static_assert(!X8 || (W4 && GATHER), "8-bit rows: gate/up and fc1 over MXFP4 weights");
-    constexpr int WCH = (W8 || (MODE == kFc2Rows && !W4)) ? 2 : 1;
-    constexpr int KSTEP = F32 ? kDvStep : (W4 ? 128 : W8 ? 64 : kDvStep) * WCH;
-    constexpr int KG = F32 ? 8 : (W4 ? 32 : W8 ? 16 : 8) * WCH;  // k per lane group per step
-    constexpr int KC = F32 ? 8 / WCH : W4 ? 32 : W8 ? 16 : 8;    // k per weight chunk
-    constexpr int WBITS = F32 ? 32 : W4 ? 4 : W8 ? 8 : 16;       // bits per weight
-    constexpr int AB = F32 ? 4 : X8 ? 1 : 2;                     // bytes per activation
-    constexpr int AH = F32 ? 2 : KG * AB / 16;                   // 16-byte A loads per row and step
+    static_assert(!F32 || (!W8 && !PK && CPL == 4), "f32: API layout, 4 columns per lane");
+    constexpr int WCH = (W8 || MODE == kFc2Rows) ? 2 : 1;
+    constexpr int KSTEP = F32 ? kDvStep : (W8 ? 64 : kDvStep) * WCH;
+    constexpr int KG = F32 ? 8 : (W8 ? 16 : 8) * WCH;  // k per lane group per step
+    constexpr int KC = F32 ? 8 / WCH : W8 ? 16 : 8;    // k per weight chunk
+    constexpr int WB = F32 ? 4 : W8 ? 1 : 2;           // bytes per weight
+    constexpr int AB = F32 ? 4 : 2;                    // bytes per activation
+    constexpr int AH = F32 ? 2 : (W8 ? 2 : 1) * WCH;   // 16-byte A loads per row and step
     constexpr bool ROWS = (MODE == kDownRows || MODE == kFc2Rows);
     constexpr int NT = 64 * kDvWaves;
     constexpr int WGC = 16 * CPL;                // output columns per workgroup
@@ -374,17 +256,9 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     const int col0 = cb * WGC;
 
     // weights of expert e (this wave's tensor): in-range loads only, zeros past
-    const long long wbytes = a.strideB * WBITS / 8;
-    const char* wbase = reinterpret_cast<const char*>(tensor ? a.B1 : a.B0) + (long long)e * wbytes;
+    const char* wbase = reinterpret_cast<const char*>(tensor ? a.B1 : a.B0) + (long long)e * a.strideB * WB;
     const __amdgpu_buffer_rsrc_t rw =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(wbase), 0, (int)wbytes, 0x00020000);
-    // (W4) the expert's scale bytes; (X8) the rows'
-    const long long sbytes = a.strideB / 32;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        W4 ? const_cast<uint8_t*>(tensor ? a.mx1 : a.mx0) + (long long)e * sbytes : nullptr, 0, W4 ? (int)sbytes : 0,
-        0x00020000);
-    const __amdgpu_buffer_rsrc_t rxs = __builtin_amdgcn_make_buffer_rsrc(
-        X8 ? const_cast<uint8_t*>(a.xs) : nullptr, 0, X8 ? (int)(a.a_bytes / 32) : 0, 0x00020000);
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(wbase), 0, (int)(a.strideB * WB), 0x00020000);
     const __amdgpu_buffer_rsrc_t rx =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.A), 0, (int)a.a_bytes, 0x00020000);
 
@@ -392,7 +266,7 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     // whole number of ring rounds (the steps past s_hi load zeros), so that
     // the ring loop needs no guard. The parts depend on K, the slices and the
     // waves only (not on the ring or the column block).
-    constexpr int RING = dec_ring<CPL, WCH, F32, W4, RB>();
+    constexpr int RING = dec_ring<CPL, WCH, F32>();
     const int nks = (K + KSTEP - 1) / KSTEP;
     const int nparts = KP * ks;
     const int per = (nks + nparts - 1) / nparts;
@@ -410,23 +284,21 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     // [N,K]: column ncol[b], k KG*g. A lane whose columns lie past N starts at
     // kOob. (Every offset stays below 2^32: kOob plus less than the expert's
     // 2^31 bytes.)
-    const uint32_t ldb2 = (uint32_t)a.ldb * (uint32_t)WBITS / 8u;  // bytes per weight row
+    const uint32_t ldb2 = (uint32_t)a.ldb * (uint32_t)WB;  // bytes per weight row
     uint32_t wlane[TRANS ? 1 : NB];
 #pragma unroll
     for (int b = 0; b < (TRANS ? 1 : NB); ++b)
-        wlane[b] = ncol[b] < N ? (TRANS ? 8u * (uint32_t)g * ldb2 + (uint32_t)(WBITS / 8) * (uint32_t)ncol[0]
-                                        : (uint32_t)ncol[b] * ldb2 + (uint32_t)(KG * WBITS / 8) * (uint32_t)g)
+        wlane[b] = ncol[b] < N ? (TRANS ? 8u * (uint32_t)g * ldb2 + (uint32_t)WB * (uint32_t)ncol[0]
+                                        : (uint32_t)ncol[b] * ldb2 + (uint32_t)(KG * WB) * (uint32_t)g)
                                : kOob;
 
     // ring of steps: weight chunks (CPL 16-bit values each for [K,N], 8 for
     // [N,K]) and the A rows. Branch-free offsets (a branch, or a select on
     // the step alone, made the compiler wait for every load in flight): a
     // lane's k positions past K read zeros (kOob).
-    constexpr int WDW = TRANS ? CPL * WBITS / 32 : 4;  // dwords per weight load
+    constexpr int WDW = TRANS ? CPL * WB / 4 : 4;  // dwords per weight load
     uint32_t wv[RING][NLD][WDW];
     u32x4 xv[RING][RB][AH];
-    uint32_t sv[W4 ? RING : 1][W4 ? NLD : 1];         // scale bytes of the chunks
-    uint32_t xsv[X8 ? RING : 1][RB][X8 ? WCH : 1];    // and of the rows' 32 k
     // this lane's k of step s, chunk c, inside the wave's part and K (K is a
     // multiple of KC: a chunk lies wholly inside or outside). Bitwise, not
     // short-circuit: a branch on the uniform s < s_hi made the compiler wait
@@ -442,9 +314,7 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
             const bool kok = k_ok(s, c);
             uint32_t o;
             if constexpr (TRANS) o = kok ? wlane[0] + (uint32_t)(s * KSTEP + t) * ldb2 : kOob;
-            else o = kok ? wlane[t / WCH] + (uint32_t)(s * (KSTEP * WBITS / 8) + 16 * c) : kOob;
-            if constexpr (W4)
-                sv[i][t] = __builtin_amdgcn_raw_buffer_load_b8(rs, kok ? o / 16u : kOob, 0, 0);
+            else o = kok ? wlane[t / WCH] + (uint32_t)(s * KSTEP * WB + 16 * c) : kOob;
             if constexpr (WDW == 4) {
                 const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rw, o, 0, 0);
 #pragma unroll
@@ -474,7 +344,7 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
     for (int c0 = 0; c0 < cnt; c0 += RB * 16) {
         const int m_valid = min(RB * 16, cnt - c0);
         // A rows of this lane (row li of each row block), k 8g
-        uint32_t abase[RB];  // (X8: a scale byte is at abase / 32)
+        uint32_t abase[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             const int m = rb * 16 + li;
@@ -505,11 +375,6 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
                     const bool kok = k_ok(s, h / (AH / WCH));
                     xv[i][rb][h] = __builtin_amdgcn_raw_buffer_load_b128(
                         rx, kok ? abase[rb] + (uint32_t)(s * KSTEP * AB) + 16u * h : kOob, 0, 0);
-                    if constexpr (X8) {
-                        if (h % 2 == 0)
-                            xsv[i][rb][h / 2] = __builtin_amdgcn_raw_buffer_load_b8(
-                                rxs, kok ? (abase[rb] + (uint32_t)(s * KSTEP)) / 32u + (uint32_t)(h / 2) : kOob, 0, 0);
-                    }
                 }
         };
         auto load = [&](int i, int st) {
@@ -527,37 +392,6 @@ __global__ __launch_bounds__(64 * kDvWaves, 2) void moe_dec_gemv(DecArgs a) {
                                         __uint_as_float(y[2]), __uint_as_float(y[3])};
                     split8(v, ap[rb][0], ap[rb][1], ap[rb][2]);
                 }
-            }
-            if constexpr (W4) {
-                // chunk c: 32 k of column b and of the row, as four operands of 8 k
-#pragma unroll
-                for (int c = 0; c < WCH; ++c) {
-                    u32x4 ao[RB][4];
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) {
-                            if constexpr (X8) {
-                                const u32x4& x = xv[i][rb][2 * c + m / 2];
-                                ao[rb][m] = mx8x8_to<DT>(u32x2{x[2 * (m & 1)], x[2 * (m & 1) + 1]},
-                                                         __uint_as_float(xsv[i][rb][c] << 23));
-                            } else {
-                                ao[rb][m] = xv[i][rb][4 * c + m];
-                            }
-                        }
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        const uint32_t(&w)[WDW] = wv[i][b * WCH + c];
-                        const float sc = __uint_as_float(sv[i][b * WCH + c] << 23);
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) {
-                            const u32x4 wo = mx4x8_to<DT>(w[m], sc);
-#pragma unroll
-                            for (int rb = 0; rb < RB; ++rb) acc[rb][b] = mfma16<DT>(ao[rb][m], wo, acc[rb][b]);
-                        }
-                    }
-                }
-                return;
             }
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -844,40 +678,26 @@ hipError_t launch_cfg(const DecArgs& a, hipStream_t stream) {
     if (a.max_groups <= 0) return hipSuccess;
     const dim3 grid((int)nwg), block(64 * kDvWaves);
     if constexpr (DT != kF32) {
-        // fp8 and MXFP4 codes are [N,K] for every GEMM (Nomic's fc2 runs the down mode)
-        constexpr int M8 = MODE == kFc2Rows ? kDownRows : MODE;
         if (a.w8) {
-            hipLaunchKernelGGL((moe_dec_gemv<DT, M8, RB, CPL, false, kDecFp8>), grid, block, 0, stream, a);
+            // fp8 codes are [N,K] for every GEMM (Nomic's fc2 runs the down mode)
+            constexpr int M8 = MODE == kFc2Rows ? kDownRows : MODE;
+            hipLaunchKernelGGL((moe_dec_gemv<DT, M8, RB, CPL, false, true>), grid, block, 0, stream, a);
             return hipGetLastError();
-        }
-        if (a.w4) {
-            // (two row blocks of 8 columns per lane would not fit 256 registers)
-            if constexpr (RB == 2 && CPL == 8) return hipErrorInvalidValue;
-            else {
-            if constexpr (M8 != kDownRows) {
-                if (a.xs) {
-                    hipLaunchKernelGGL((moe_dec_gemv<DT, M8, RB, CPL, false, kDecMxfp4, true>), grid, block, 0, stream, a);
-                    return hipGetLastError();
-                }
-            }
-            hipLaunchKernelGGL((moe_dec_gemv<DT, M8, RB, CPL, false, kDecMxfp4>), grid, block, 0, stream, a);
-            return hipGetLastError();
-            }
         }
     }
     if constexpr (DT == kF32) {
-        hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, false, 0>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, false, false>), grid, block, 0, stream, a);
         return hipGetLastError();
     }
     // (Nomic's fc2 is [N,K] either way: no packed instance)
     if constexpr (MODE != kFc2Rows && DT != kF32) {
         if (a.packed) {
-            hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, true, 0>), grid, block, 0, stream, a);
+            hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, true, false>), grid, block, 0, stream, a);
             return hipGetLastError();
         }
     }
     if constexpr (DT != kF32 && (MODE == kFc2Rows || (CPL != 3 && CPL != 6))) {
-        hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, false, 0>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((moe_dec_gemv<DT, MODE, RB, CPL, false, false>), grid, block, 0, stream, a);
         return hipGetLastError();
     }
     return hipErrorInvalidValue;  // [K,N] weights: 2, 4 or 8 columns per lane

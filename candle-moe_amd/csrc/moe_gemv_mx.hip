@@ -1,0 +1,337 @@
+// Decode GEMMs over MXFP4 expert weights (gfx950): few rows per touched expert, so
+// the time is the weight stream (4.25 bits a weight) and the latency around it.
+//
+// As in moe_gemv_dec.hip a workgroup finds its item (touched expert, block of
+// 16 * CPL columns) and the expert's pairs itself, its 4 waves split K (gate/up:
+// two waves per tensor), weights go straight into registers and the parts meet
+// through LDS once, in a fixed order. What differs:
+//  * A step is 128 k: lane (g, i) (g = lane / 16, i = lane % 16) loads the 16
+//    bytes that hold k0 + 32 g .. +31 of its column and their one scale byte. The
+//    gfx950 scaled conversions turn 8 codes and the scale into an operand of
+//    v_mfma_f32_16x16x32, exactly in bf16: no weight is rounded, no sum rescaled.
+//  * The expert's rows go through LDS (DMA, once per workgroup), so that a wave's
+//    registers hold weights only and a whole K part of up to RING steps is in
+//    flight at once. With the rows in the same registers, in flight next to the
+//    weights, a step took twice the registers and the ring was half as long: Qwen3
+//    T=16 gate/up 19.2, Qwen3-30B-A3B T=1 8.5 us (one wave per SIMD and item: the
+//    time of a launch is its trips to memory).
+//  * Rows are 16-bit or MXFP8 (X8: e4m3 codes through LDS, a scale byte per row and
+//    step beside the weights'), converted the same way.
+// Rows of a tile are padded by 16 bytes in LDS: 16 lanes reading 16 rows at one k
+// land in different banks. K chunks (DecArgs::kc) bound the LDS of long rows.
+#include <algorithm>
+
+#include "cm_dec.hpp"
+
+namespace cm {
+
+using namespace lds;
+using namespace dec;
+
+namespace {
+
+constexpr int kMxWaves = 4;
+
+// Weight steps in flight per wave: about 120 registers of them, so that two
+// workgroups share a CU where their LDS lets them.
+template <int CPL>
+constexpr int mx_ring() { return CPL <= 3 ? 8 : CPL == 4 ? 6 : CPL == 6 ? 4 : 3; }
+
+template <int DT, int MODE, int RB, int CPL, bool X8>
+__global__ __launch_bounds__(64 * kMxWaves, 2) void mx_dec_k(DecArgs a) {
+    constexpr bool DUAL = (MODE == kGateUp);
+    constexpr bool GATHER = (MODE == kGateUp || MODE == kFc1);
+    static_assert(GATHER || !X8, "8-bit rows: gate/up and fc1");
+    constexpr int NT = 64 * kMxWaves, KP = DUAL ? kMxWaves / 2 : kMxWaves, RING = mx_ring<CPL>();
+    constexpr int WGC = 16 * CPL, SPW = WGC + 4, AB = X8 ? 1 : 2;
+
+    __shared__ uint32_t s_bm[kDecMaxE / 32];
+    __shared__ int32_t s_idx[kDecMaxPairs];
+    __shared__ int32_t s_rows[kDecMaxPairs];
+    __shared__ int s_misc[8 + kMxWaves];
+    // rows of the expert, then (after the K loop) the waves' parts [wave][row][SPW]
+    extern __shared__ __attribute__((aligned(16))) char s_dyn[];
+    float* s_part = reinterpret_cast<float*>(s_dyn);
+
+    int e, cb, cnt = 0;
+    const bool few = a.P <= 64;
+    if (few) {
+        cnt = dec_assign64(a, GATHER ? 0 : 1, s_rows, e, cb);
+    } else {
+        dec_assign<NT, false>(a, GATHER ? 0 : 1, s_bm, s_idx, s_misc);
+        e = s_misc[0];
+        cb = s_misc[1];
+    }
+    if (e < 0) return;
+    if (!few) cnt = dec_rows<NT>(a, e, s_idx, s_rows, s_misc);
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, li = lane & 15;
+    const int tensor = DUAL ? wave / KP : 0;
+    const int kpart = DUAL ? wave - tensor * KP : wave;
+    const int K = a.K, N = a.N, col0 = cb * WGC;
+
+    // codes and scale bytes of expert e (in-range loads only, zeros past), the rows
+    const long long wbytes = a.strideB / 2, sbytes = a.strideB / 32;
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(reinterpret_cast<const char*>(tensor ? a.B1 : a.B0)) + (long long)e * wbytes, 0, (int)wbytes,
+        0x00020000);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(tensor ? a.mx1 : a.mx0) + (long long)e * sbytes, 0, (int)sbytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rxs = __builtin_amdgcn_make_buffer_rsrc(
+        X8 ? const_cast<uint8_t*>(a.xs) : nullptr, 0, X8 ? (int)(a.a_bytes / 32) : 0, 0x00020000);
+    const i32x4 rA = make_rsrc(a.A, a.a_bytes);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(s_dyn));
+
+    // first byte of this lane's codes in each column block (its scale byte is at a
+    // sixteenth of that); past N: out of range
+    uint32_t wlane[CPL];
+#pragma unroll
+    for (int b = 0; b < CPL; ++b) {
+        const int n = col0 + 16 * b + li;
+        wlane[b] = n < N ? (uint32_t)n * (uint32_t)(K / 2) + 16u * (uint32_t)g : kOob;
+    }
+
+    for (int c0 = 0; c0 < cnt; c0 += RB * 16) {
+        const int m_valid = min(RB * 16, cnt - c0);
+        f32x4 acc[RB][CPL];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int b = 0; b < CPL; ++b) acc[rb][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        uint32_t xs0[X8 ? RB : 1];  // first scale byte of this lane's rows
+        if constexpr (X8) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const int p = s_rows[c0 + min(rb * 16 + li, m_valid - 1)];
+                xs0[rb] = (uint32_t)(p / a.k_top) * (uint32_t)(K / 32) + (uint32_t)g;
+            }
+        }
+
+        for (int k0 = 0; k0 < K; k0 += a.kc) {
+            const int kn = min(a.kc, K - k0);  // k of this chunk
+            const int segs = (kn * AB + 1023) >> 10;
+            const int pitch = segs * 1024 + 16;
+            if (k0 > 0 || c0 > 0) __syncthreads();  // (the LDS is read no more)
+            // rows to LDS: one instruction per 1 KB, the waves in turn
+            for (int q = wave; q < m_valid * segs; q += kMxWaves) {
+                const int r = q / segs, sg = q - r * segs;
+                const int p = __builtin_amdgcn_readfirstlane(s_rows[c0 + r]);
+                const uint32_t row = (uint32_t)(GATHER ? p / a.k_top : p) * (uint32_t)(K * AB) + (uint32_t)(k0 * AB);
+                const uint32_t at = (uint32_t)sg * 1024u + 16u * (uint32_t)lane;
+                dma16(rA, lds0 + (uint32_t)(r * pitch + sg * 1024), at < (uint32_t)(kn * AB) ? row + at : kOob);
+            }
+
+            // this wave's steps of the chunk
+            const int nks = (kn + 127) / 128, per = (nks + KP - 1) / KP;
+            const int s_lo = kpart * per, n = min(per, nks - s_lo);
+            u32x4 wv[RING][CPL];
+            uint32_t sv[RING][CPL];
+            uint32_t xv[X8 ? RING : 1][X8 ? RB : 1];
+            auto load = [&](int i, int st) {
+                const int k = k0 + (s_lo + st) * 128;
+                const bool in = (st < n) & (k + 32 * g < k0 + kn);  // (K is a multiple of 32: whole chunks)
+#pragma unroll
+                for (int b = 0; b < CPL; ++b) {
+                    const uint32_t o = in ? wlane[b] + (uint32_t)(k / 2) : kOob;
+                    wv[i][b] = __builtin_amdgcn_raw_buffer_load_b128(rw, o, 0, 0);
+                    sv[i][b] = __builtin_amdgcn_raw_buffer_load_b8(rs, in ? o / 16u : kOob, 0, 0);
+                }
+                if constexpr (X8) {
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb)
+                        xv[i][rb] = __builtin_amdgcn_raw_buffer_load_b8(rxs, in ? xs0[rb] + (uint32_t)(k / 32) : kOob, 0, 0);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < RING; ++i) load(i, i);
+            // the rows are older than the RING steps' loads
+            constexpr int LOADS = RING * (2 * CPL + (X8 ? RB : 0));
+            wait_vm<(LOADS < 63 ? LOADS : 63)>();
+            block_barrier();
+
+            uint32_t arow[RB];  // byte of this lane's k in its rows (rows past the last: the last)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+                arow[rb] = (uint32_t)(min(rb * 16 + li, m_valid - 1) * pitch + 32 * AB * g);
+            auto compute = [&](int i, int st) {
+                u32x4 ao[RB][4];
+                const uint32_t ka = (uint32_t)((s_lo + st) * 128 * AB);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    const u32x4* src = reinterpret_cast<const u32x4*>(s_dyn + arow[rb] + ka);
+                    if constexpr (X8) {
+                        const u32x4 v0 = src[0], v1 = src[1];
+                        const float sc = __uint_as_float(xv[i][rb] << 23);
+                        ao[rb][0] = mx8x8_to<DT>(u32x2{v0[0], v0[1]}, sc);
+                        ao[rb][1] = mx8x8_to<DT>(u32x2{v0[2], v0[3]}, sc);
+                        ao[rb][2] = mx8x8_to<DT>(u32x2{v1[0], v1[1]}, sc);
+                        ao[rb][3] = mx8x8_to<DT>(u32x2{v1[2], v1[3]}, sc);
+                    } else {
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) ao[rb][m] = src[m];
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < CPL; ++b) {
+                    const float sc = __uint_as_float(sv[i][b] << 23);
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        const u32x4 wo = mx4x8_to<DT>(wv[i][b][m], sc);
+#pragma unroll
+                        for (int rb = 0; rb < RB; ++rb) acc[rb][b] = mfma16<DT>(ao[rb][m], wo, acc[rb][b]);
+                    }
+                }
+            };
+            // full rounds, each step's slot refilled behind it; then what is left,
+            // one branch inside the other (a join would wait for every load)
+            int st = 0;
+            for (; st + RING < n; st += RING) {
+#pragma unroll
+                for (int i = 0; i < RING; ++i) {
+                    compute(i, st + i);
+                    __builtin_amdgcn_sched_barrier(0);
+                    load(i, st + i + RING);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            auto rest = [&](auto self, auto ic) -> void {
+                constexpr int i = decltype(ic)::value;
+                if constexpr (i < RING) {
+                    if (st + i < n) {
+                        compute(i, st + i);
+                        __builtin_amdgcn_sched_barrier(0);
+                        self(self, std::integral_constant<int, i + 1>{});
+                    }
+                }
+            };
+            rest(rest, std::integral_constant<int, 0>{});
+        }
+
+        // parts to LDS: lane (g, li) holds rows 4g .. 4g+3 of each row block at
+        // column 16b + li
+        __syncthreads();
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int b = 0; b < CPL; ++b)
+                    s_part[(wave * RB * 16 + rb * 16 + 4 * g + v) * SPW + 16 * b + li] = acc[rb][b][v];
+        __syncthreads();
+        // every thread: 8 consecutive columns of one row, the parts in wave order
+        auto part_sums = [&](int m, int c8, int tn, float (&y)[8]) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                f32x4 v = *reinterpret_cast<const f32x4*>(s_part + (tn * KP * RB * 16 + m) * SPW + c8 + 4 * half);
+#pragma unroll
+                for (int pt = 1; pt < KP; ++pt) {
+                    const f32x4 w =
+                        *reinterpret_cast<const f32x4*>(s_part + ((tn * KP + pt) * RB * 16 + m) * SPW + c8 + 4 * half);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] += w[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[4 * half + j] = v[j];
+            }
+        };
+        constexpr int CH = WGC / 8;
+        // (N is a multiple of 32: 8 columns lie wholly inside or outside)
+        if constexpr (GATHER) {
+            with_act(a.act, [&](auto act_c) {
+                constexpr int ACT = decltype(act_c)::value;
+                for (int q = tid; q < m_valid * CH; q += NT) {
+                    const int m = q / CH, c8 = (q - m * CH) * 8;
+                    if (col0 + c8 >= N) continue;
+                    float y0[8], y1[8], h[8];
+                    part_sums(m, c8, 0, y0);
+                    if constexpr (DUAL) part_sums(m, c8, 1, y1);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[j] = DUAL ? act_t<ACT>(y0[j]) * y1[j] : act_t<ACT>(y0[j]);
+                    u32x4 o;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j] = pack2<DT>(h[2 * j], h[2 * j + 1]);
+                    *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(a.C) + (long long)s_rows[c0 + m] * N + col0 + c8) = o;
+                }
+            });
+        } else {
+            for (int q = tid; q < m_valid * CH; q += NT) {
+                const int m = q / CH, c8 = (q - m * CH) * 8;
+                if (col0 + c8 >= N) continue;
+                float y[8];
+                part_sums(m, c8, 0, y);
+                float* dst = a.part + (long long)s_rows[c0 + m] * N + col0 + c8;
+                *reinterpret_cast<f32x4*>(dst) = f32x4{y[0], y[1], y[2], y[3]};
+                *reinterpret_cast<f32x4*>(dst + 4) = f32x4{y[4], y[5], y[6], y[7]};
+            }
+        }
+    }
+}
+
+template <int DT, int MODE, int RB, int CPL, bool X8>
+hipError_t launch_one(const DecArgs& a, hipStream_t stream) {
+    const long long nwg = (long long)a.max_groups * a.nblk;
+    if (nwg > 0x7fffffffLL) return hipErrorInvalidValue;
+    if (nwg <= 0) return hipSuccess;
+    // LDS: the rows of one chunk, or the waves' parts
+    constexpr int AB = X8 ? 1 : 2;
+    // (a token may name one expert in several slots: up to P rows)
+    const int rows = std::min(a.P, 16 * RB);
+    const int pitch = (std::min(a.kc, a.K) * AB + 1023) / 1024 * 1024 + 16;
+    const int part = kMxWaves * RB * 16 * (16 * CPL + 4) * 4;
+    const int lds = std::max(rows * pitch, part);
+    if (lds > kMxDecLds) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((mx_dec_k<DT, MODE, RB, CPL, X8>), dim3((unsigned)nwg), dim3(64 * kMxWaves), lds, stream, a);
+    return hipGetLastError();
+}
+template <int DT, int MODE, int RB, bool X8>
+hipError_t launch_cols(const DecArgs& a, hipStream_t stream) {
+    switch (a.cpl) {
+        case 2: return launch_one<DT, MODE, RB, 2, X8>(a, stream);
+        case 3: return launch_one<DT, MODE, RB, 3, X8>(a, stream);
+        case 4: return launch_one<DT, MODE, RB, 4, X8>(a, stream);
+        case 6: return launch_one<DT, MODE, RB, 6, X8>(a, stream);
+        case 8:
+            if constexpr (RB == 1) return launch_one<DT, MODE, RB, 8, X8>(a, stream);
+            return hipErrorInvalidValue;
+        default: return hipErrorInvalidValue;
+    }
+}
+template <int DT, int MODE>
+hipError_t launch_mode(const DecArgs& a, hipStream_t stream) {
+    if constexpr (MODE != kDownRows) {
+        if (a.xs) return a.rows_max > 16 ? launch_cols<DT, MODE, 2, true>(a, stream) : launch_cols<DT, MODE, 1, true>(a, stream);
+    }
+    return a.rows_max > 16 ? launch_cols<DT, MODE, 2, false>(a, stream) : launch_cols<DT, MODE, 1, false>(a, stream);
+}
+template <int DT>
+hipError_t launch_dt(int mode, const DecArgs& a, hipStream_t stream) {
+    switch (mode) {
+        case kGateUp: return launch_mode<DT, kGateUp>(a, stream);
+        case kFc1: return launch_mode<DT, kFc1>(a, stream);
+        case kDownRows:
+        case kFc2Rows: return launch_mode<DT, kDownRows>(a, stream);  // ([N,K] either way)
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+int mx_dec_chunk(int rows_max, int K, int row_bytes) {
+    // whole steps for every wave, and rows of 1 KB in LDS (512 k of 16 bits)
+    const int rows = rows_max > 16 ? 32 : 16;
+    const int most = (kMxDecLds / rows - 16) / 1024 * 1024 / row_bytes;
+    return K <= most ? (K + 511) / 512 * 512 : most / 1024 * 1024;
+}
+
+hipError_t launch_mx_dec(int mode, int dtype, const DecArgs& a, hipStream_t stream) {
+    if (a.P > kDecMaxPairs || a.E > kDecMaxE || a.ks_lim != 1 || a.meta == nullptr || a.mx0 == nullptr ||
+        (mode == kGateUp && a.mx1 == nullptr) || a.kc < 512 || a.kc % 512 || a.K % 32 || a.N % 32)
+        return hipErrorInvalidValue;
+    if (dtype == kBF16) return launch_dt<kBF16>(mode, a, stream);
+    if (dtype == kF16) return launch_dt<kF16>(mode, a, stream);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace cm
