@@ -315,6 +315,7 @@ static Layout make_layout(const Problem& p) {
 // up to 512 past K: the weight offsets stay below 2^31 with that margin.)
 static bool dec_gemv_fits(const Problem& p) {
     const long long lim = 0x7fffff00LL, es = p.dtype == kF32 ? 4 : 2;
+    if (p.mx && (p.H > kMxDecMaxK || p.I > kMxDecMaxK)) return false;
     return (p.mfma || p.f32_dec) && p.P <= kDecMaxPairs && p.E <= kDecMaxE && (long long)p.T * p.H * es < lim &&
            p.P * p.I * es < lim && p.P * p.H * es < lim && (long long)(p.H + 1024) * p.I * es < lim &&
            (long long)(p.I + 1024) * p.H * es < lim;
@@ -880,7 +881,6 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
         d.mx0 = mx->gate_s;
         d.mx1 = mx->up_s;
         d.xs = mx->x_s;
-        d.kc = mx_dec_chunk((int)std::min<long long>(p.P, p.T), p.H, mx->x_s ? 1 : 2);
     }
     const int es = p.dtype == kF32 ? 4 : 2;
     d.a_bytes = (long long)p.T * p.H * (mx && mx->x_s ? 1 : es);
@@ -888,8 +888,8 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     d.rows_max = (int)std::min<long long>(p.P, p.T);
     d.cap = dec_cap();
     d.ks_lim = p.dec_ks1;
-    const int most_cpl = mx && d.rows_max > 16 ? 6 : 8;  // (launch_mx_dec)
-    d.cpl = dec_cpl(d.max_groups, p.I, !nk, d.ks_lim, p.dtype == kF32, most_cpl);
+    d.cpl = dec_cpl(d.max_groups, p.I, !nk, d.ks_lim, p.dtype == kF32,
+                    mx ? mx_dec_cols(qwen3 ? kGateUp : kFc1, d.rows_max, p.H) : 8);
     d.nblk = cdiv(p.I, 16 * d.cpl);
     const int mode1 = qwen3 ? kGateUp : kFc1;
     hipError_t e;
@@ -926,7 +926,6 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     if (mx) {
         d2.mx0 = qwen3 ? mx->down_s : mx->up_s;
         d2.mx1 = d2.xs = nullptr;
-        d2.kc = mx_dec_chunk(d.rows_max, p.I, 2);
     }
     d2.a_bytes = p.P * p.I * es;
     d2.ks_lim = p.dec_ks2;
@@ -935,7 +934,8 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     const float* s2 = f8 ? (qwen3 ? f8->down_scale : f8->up_scale) : nullptr;
     d2.scale0 = d2.ks_lim == 1 ? s2 : nullptr;
     d2.scale1 = nullptr;
-    d2.cpl = dec_cpl(d.max_groups, p.H, qwen3 && !nk, d2.ks_lim, p.dtype == kF32, most_cpl);
+    d2.cpl = dec_cpl(d.max_groups, p.H, qwen3 && !nk, d2.ks_lim, p.dtype == kF32,
+                     mx ? mx_dec_cols(kDownRows, d.rows_max, p.I) : 8);
     d2.nblk = cdiv(p.H, 16 * d2.cpl);
     {
         ProfScope ps(kSlotGemm2, s);

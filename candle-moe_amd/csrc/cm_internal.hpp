@@ -352,14 +352,15 @@ struct DecArgs {
     const uint8_t* mx0;       // launch_mx_dec: scale bytes [E][N][K/32] of B0 (codes [E][N][K/2])
     const uint8_t* mx1;       // and of B1
     const uint8_t* xs;        // (kGateUp / kFc1) A is MXFP8 codes: their scale bytes [T][K/32], else null
-    int kc;                   // k of a row staged in LDS at a time (mx_dec_chunk)
+    int kc, lds_rows;         // k of a row staged in LDS at a time, its place (set by the launch)
 };
 hipError_t launch_dec_gemv(int mode, int dtype, const DecArgs& a, hipStream_t stream);
 // Decode GEMMs over MXFP4 weights (moe_gemv_mx.hip): kGateUp, kFc1 (inter [P, N] by
 // pair in the dtype), kDownRows / kFc2Rows (f32 partials, one slice); ks_lim 1,
-// cpl 2, 3, 4, 6 or (rows_max <= 16) 8.
-constexpr int kMxDecLds = 144 * 1024;
-int mx_dec_chunk(int rows_max, int K, int row_bytes);
+// cpl 2, 3, 4, 6 or 8, at most mx_dec_cols(); K up to kMxDecMaxK.
+constexpr int kMxDecLds = 150 * 1024;
+constexpr int kMxDecMaxK = 16384;
+int mx_dec_cols(int mode, int rows_max, int K);
 hipError_t launch_mx_dec(int mode, int dtype, const DecArgs& a, hipStream_t stream);
 // Finishing the K slices of a decode GEMM (fixed slice order: deterministic),
 // ks = meta[0] (gate/up, fc1) or meta[1] (down, fc2), as the GEMM stored it.

@@ -6,17 +6,21 @@
 // two waves per tensor), weights go straight into registers and the parts meet
 // through LDS once, in a fixed order. What differs:
 //  * A step is 128 k: lane (g, i) (g = lane / 16, i = lane % 16) loads the 16
-//    bytes that hold k0 + 32 g .. +31 of its column and their one scale byte. The
+//    bytes that hold k0 + 32 g .. +31 of its column, which share one scale byte. The
 //    gfx950 scaled conversions turn 8 codes and the scale into an operand of
 //    v_mfma_f32_16x16x32, exactly in bf16: no weight is rounded, no sum rescaled.
+//  * The block's scale bytes are one contiguous piece of memory and come through
+//    LDS. (A byte load per lane beside every code load cost more than the codes:
+//    loads alone, Qwen3 T=16 gate/up 16.5 against 12.0 us, Qwen3-30B-A3B T=1 7.4
+//    against 5.8.)
 //  * The expert's rows go through LDS (DMA, once per workgroup), so that a wave's
 //    registers hold weights only and a whole K part of up to RING steps is in
 //    flight at once. With the rows in the same registers, in flight next to the
 //    weights, a step took twice the registers and the ring was half as long: Qwen3
 //    T=16 gate/up 19.2, Qwen3-30B-A3B T=1 8.5 us (one wave per SIMD and item: the
 //    time of a launch is its trips to memory).
-//  * Rows are 16-bit or MXFP8 (X8: e4m3 codes through LDS, a scale byte per row and
-//    step beside the weights'), converted the same way.
+//  * Rows are 16-bit or MXFP8 (X8: e4m3 codes and their scale bytes through LDS),
+//    converted the same way.
 // Rows of a tile are padded by 16 bytes in LDS: 16 lanes reading 16 rows at one k
 // land in different banks. K chunks (DecArgs::kc) bound the LDS of long rows.
 #include <algorithm>
@@ -49,9 +53,12 @@ __global__ __launch_bounds__(64 * kMxWaves, 2) void mx_dec_k(DecArgs a) {
     __shared__ int32_t s_idx[kDecMaxPairs];
     __shared__ int32_t s_rows[kDecMaxPairs];
     __shared__ int s_misc[8 + kMxWaves];
-    // rows of the expert, then (after the K loop) the waves' parts [wave][row][SPW]
+    // scale bytes of the block's columns (of both tensors), those of the rows (X8);
+    // from a.lds_rows on the expert's rows, after the K loop the waves' parts
+    // [wave][row][SPW]
     extern __shared__ __attribute__((aligned(16))) char s_dyn[];
-    float* s_part = reinterpret_cast<float*>(s_dyn);
+    char* s_a = s_dyn + a.lds_rows;
+    float* s_part = reinterpret_cast<float*>(s_a);
 
     int e, cb, cnt = 0;
     const bool few = a.P <= 64;
@@ -74,18 +81,28 @@ __global__ __launch_bounds__(64 * kMxWaves, 2) void mx_dec_k(DecArgs a) {
 
     // codes and scale bytes of expert e (in-range loads only, zeros past), the rows
     const long long wbytes = a.strideB / 2, sbytes = a.strideB / 32;
+    const int kb = K / 32, sblock = WGC * kb;  // scale bytes of a column, of the block
+    const int sround = (sblock + 1023) & ~1023;
     const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<char*>(reinterpret_cast<const char*>(tensor ? a.B1 : a.B0)) + (long long)e * wbytes, 0, (int)wbytes,
         0x00020000);
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(tensor ? a.mx1 : a.mx0) + (long long)e * sbytes, 0, (int)sbytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rxs = __builtin_amdgcn_make_buffer_rsrc(
-        X8 ? const_cast<uint8_t*>(a.xs) : nullptr, 0, X8 ? (int)(a.a_bytes / 32) : 0, 0x00020000);
     const i32x4 rA = make_rsrc(a.A, a.a_bytes);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(s_dyn));
 
-    // first byte of this lane's codes in each column block (its scale byte is at a
-    // sixteenth of that); past N: out of range
+    // the block's scales, 1 KB per instruction, the waves of a tensor in turn (past
+    // the expert's matrix: zeros)
+    {
+        const long long se = (long long)e * sbytes;
+        const i32x4 rs = make_rsrc((tensor ? a.mx1 : a.mx0) + se, sbytes);
+        for (int q = kpart; q < sround >> 10; q += KP)
+            dma16(rs, lds0 + (uint32_t)(tensor * sround + q * 1024),
+                  (uint32_t)col0 * (uint32_t)kb + (uint32_t)q * 1024u + 16u * (uint32_t)lane);
+    }
+    const uint8_t* s_sc = reinterpret_cast<const uint8_t*>(s_dyn) + tensor * sround + li * kb + g;
+    const int xp = (kb + 255) & ~255;  // (X8) LDS pitch of a row's scale bytes
+    uint8_t* s_xs = reinterpret_cast<uint8_t*>(s_dyn) + (DUAL ? 2 : 1) * sround;
+
+    // first byte of this lane's codes in each column block; past N: out of range
     uint32_t wlane[CPL];
 #pragma unroll
     for (int b = 0; b < CPL; ++b) {
@@ -100,55 +117,56 @@ __global__ __launch_bounds__(64 * kMxWaves, 2) void mx_dec_k(DecArgs a) {
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
             for (int b = 0; b < CPL; ++b) acc[rb][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-        uint32_t xs0[X8 ? RB : 1];  // first scale byte of this lane's rows
-        if constexpr (X8) {
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-                const int p = s_rows[c0 + min(rb * 16 + li, m_valid - 1)];
-                xs0[rb] = (uint32_t)(p / a.k_top) * (uint32_t)(K / 32) + (uint32_t)g;
-            }
-        }
-
         for (int k0 = 0; k0 < K; k0 += a.kc) {
             const int kn = min(a.kc, K - k0);  // k of this chunk
             const int segs = (kn * AB + 1023) >> 10;
             const int pitch = segs * 1024 + 16;
             if (k0 > 0 || c0 > 0) __syncthreads();  // (the LDS is read no more)
+            if constexpr (X8) {
+                if (k0 == 0 && kb % 4 == 0 && (reinterpret_cast<uintptr_t>(a.xs) & 3) == 0) {
+                    // 256 bytes per instruction
+                    const i32x4 rx = make_rsrc(a.xs, a.a_bytes / 32);
+                    const int xsegs = xp >> 8;
+                    for (int q = wave; q < m_valid * xsegs; q += kMxWaves) {
+                        const int r = q / xsegs, at = (q - r * xsegs) * 256;
+                        const uint32_t row = (uint32_t)(__builtin_amdgcn_readfirstlane(s_rows[c0 + r]) / a.k_top) * (uint32_t)kb;
+                        dma4(rx, lds0 + (uint32_t)((DUAL ? 2 : 1) * sround + r * xp + at),
+                             at + 4 * lane < kb ? row + (uint32_t)(at + 4 * lane) : kOob);
+                    }
+                } else if (k0 == 0) {
+                    for (int q = tid; q < m_valid * kb; q += NT) {
+                        const int r = q / kb;
+                        s_xs[r * xp + (q - r * kb)] = a.xs[(long long)(s_rows[c0 + r] / a.k_top) * kb + (q - r * kb)];
+                    }
+                }
+            }
             // rows to LDS: one instruction per 1 KB, the waves in turn
             for (int q = wave; q < m_valid * segs; q += kMxWaves) {
                 const int r = q / segs, sg = q - r * segs;
                 const int p = __builtin_amdgcn_readfirstlane(s_rows[c0 + r]);
                 const uint32_t row = (uint32_t)(GATHER ? p / a.k_top : p) * (uint32_t)(K * AB) + (uint32_t)(k0 * AB);
                 const uint32_t at = (uint32_t)sg * 1024u + 16u * (uint32_t)lane;
-                dma16(rA, lds0 + (uint32_t)(r * pitch + sg * 1024), at < (uint32_t)(kn * AB) ? row + at : kOob);
+                dma16(rA, lds0 + (uint32_t)(a.lds_rows + r * pitch + sg * 1024), at < (uint32_t)(kn * AB) ? row + at : kOob);
             }
 
             // this wave's steps of the chunk
             const int nks = (kn + 127) / 128, per = (nks + KP - 1) / KP;
             const int s_lo = kpart * per, n = min(per, nks - s_lo);
             u32x4 wv[RING][CPL];
-            uint32_t sv[RING][CPL];
-            uint32_t xv[X8 ? RING : 1][X8 ? RB : 1];
             auto load = [&](int i, int st) {
                 const int k = k0 + (s_lo + st) * 128;
                 const bool in = (st < n) & (k + 32 * g < k0 + kn);  // (K is a multiple of 32: whole chunks)
 #pragma unroll
-                for (int b = 0; b < CPL; ++b) {
-                    const uint32_t o = in ? wlane[b] + (uint32_t)(k / 2) : kOob;
-                    wv[i][b] = __builtin_amdgcn_raw_buffer_load_b128(rw, o, 0, 0);
-                    sv[i][b] = __builtin_amdgcn_raw_buffer_load_b8(rs, in ? o / 16u : kOob, 0, 0);
-                }
-                if constexpr (X8) {
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb)
-                        xv[i][rb] = __builtin_amdgcn_raw_buffer_load_b8(rxs, in ? xs0[rb] + (uint32_t)(k / 32) : kOob, 0, 0);
-                }
+                for (int b = 0; b < CPL; ++b)
+                    wv[i][b] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? wlane[b] + (uint32_t)(k / 2) : kOob, 0, 0);
             };
 #pragma unroll
             for (int i = 0; i < RING; ++i) load(i, i);
-            // the rows are older than the RING steps' loads
-            constexpr int LOADS = RING * (2 * CPL + (X8 ? RB : 0));
-            wait_vm<(LOADS < 63 ? LOADS : 63)>();
+            // the rows and scales are older than the RING steps' loads
+            constexpr int LOADS = RING * CPL;
+            static_assert(LOADS < 63, "vmcnt range");
+            wait_vm<LOADS>();
+            wait_lgkm0();
             block_barrier();
 
             uint32_t arow[RB];  // byte of this lane's k in its rows (rows past the last: the last)
@@ -158,12 +176,16 @@ __global__ __launch_bounds__(64 * kMxWaves, 2) void mx_dec_k(DecArgs a) {
             auto compute = [&](int i, int st) {
                 u32x4 ao[RB][4];
                 const uint32_t ka = (uint32_t)((s_lo + st) * 128 * AB);
+                const int kq = k0 / 32 + (s_lo + st) * 4;  // (its lane group's 32 k: + g)
+                // past K the codes are zeros, and a foreign scale could be a NaN
+                const bool in = kq + g < kb;
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) {
-                    const u32x4* src = reinterpret_cast<const u32x4*>(s_dyn + arow[rb] + ka);
+                    const u32x4* src = reinterpret_cast<const u32x4*>(s_a + arow[rb] + ka);
                     if constexpr (X8) {
                         const u32x4 v0 = src[0], v1 = src[1];
-                        const float sc = __uint_as_float(xv[i][rb] << 23);
+                        const uint32_t xb = s_xs[min(rb * 16 + li, m_valid - 1) * xp + min(kq + g, kb - 1)];
+                        const float sc = __uint_as_float(xb << 23);
                         ao[rb][0] = mx8x8_to<DT>(u32x2{v0[0], v0[1]}, sc);
                         ao[rb][1] = mx8x8_to<DT>(u32x2{v0[2], v0[3]}, sc);
                         ao[rb][2] = mx8x8_to<DT>(u32x2{v1[0], v1[1]}, sc);
@@ -175,7 +197,8 @@ __global__ __launch_bounds__(64 * kMxWaves, 2) void mx_dec_k(DecArgs a) {
                 }
 #pragma unroll
                 for (int b = 0; b < CPL; ++b) {
-                    const float sc = __uint_as_float(sv[i][b] << 23);
+                    const uint32_t sb = s_sc[b * 16 * kb + kq];
+                    const float sc = __uint_as_float((in ? sb : 127u) << 23);
 #pragma unroll
                     for (int m = 0; m < 4; ++m) {
                         const u32x4 wo = mx4x8_to<DT>(wv[i][b][m], sc);
@@ -274,15 +297,22 @@ hipError_t launch_one(const DecArgs& a, hipStream_t stream) {
     const long long nwg = (long long)a.max_groups * a.nblk;
     if (nwg > 0x7fffffffLL) return hipErrorInvalidValue;
     if (nwg <= 0) return hipSuccess;
-    // LDS: the rows of one chunk, or the waves' parts
-    constexpr int AB = X8 ? 1 : 2;
-    // (a token may name one expert in several slots: up to P rows)
-    const int rows = std::min(a.P, 16 * RB);
-    const int pitch = (std::min(a.kc, a.K) * AB + 1023) / 1024 * 1024 + 16;
-    const int part = kMxWaves * RB * 16 * (16 * CPL + 4) * 4;
-    const int lds = std::max(rows * pitch, part);
+    // LDS: scales, then the rows of one chunk or the waves' parts. (A token may name
+    // one expert in several slots: up to P rows.)
+    constexpr int AB = X8 ? 1 : 2, PART = kMxWaves * RB * 16 * (16 * CPL + 4) * 4;
+    const long long rows = std::min(a.P, 16 * RB), kb = a.K / 32;
+    const long long scales = (MODE == kGateUp ? 2 : 1) * ((16 * CPL * kb + 1023) / 1024 * 1024);
+    const long long first = scales + (X8 ? rows * ((kb + 255) / 256 * 256) : 0);
+    const long long most = ((kMxDecLds - first) / rows - 16) / 1024 * 1024 / AB;  // k of the rows that fit
+    if (first + PART > kMxDecLds || most < 512) return hipErrorInvalidValue;
+    DecArgs b = a;
+    b.lds_rows = (int)first;
+    const long long chunks = (a.K + most - 1) / most;
+    b.kc = (int)(((a.K + chunks - 1) / chunks + 511) / 512 * 512);
+    const long long pitch = ((long long)std::min(b.kc, a.K) * AB + 1023) / 1024 * 1024 + 16;
+    const long long lds = first + std::max<long long>(rows * pitch, PART);
     if (lds > kMxDecLds) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((mx_dec_k<DT, MODE, RB, CPL, X8>), dim3((unsigned)nwg), dim3(64 * kMxWaves), lds, stream, a);
+    hipLaunchKernelGGL((mx_dec_k<DT, MODE, RB, CPL, X8>), dim3((unsigned)nwg), dim3(64 * kMxWaves), (unsigned)lds, stream, b);
     return hipGetLastError();
 }
 template <int DT, int MODE, int RB, bool X8>
@@ -318,16 +348,15 @@ hipError_t launch_dt(int mode, const DecArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int mx_dec_chunk(int rows_max, int K, int row_bytes) {
-    // whole steps for every wave, and rows of 1 KB in LDS (512 k of 16 bits)
-    const int rows = rows_max > 16 ? 32 : 16;
-    const int most = (kMxDecLds / rows - 16) / 1024 * 1024 / row_bytes;
-    return K <= most ? (K + 511) / 512 * 512 : most / 1024 * 1024;
+int mx_dec_cols(int mode, int rows_max, int K) {
+    // (two row blocks of 8 columns do not fit 256 registers; scales at most 32 KB)
+    const int most = (mode == kGateUp ? 1 : 2) * 32768 / K;
+    return std::min(rows_max > 16 ? 6 : 8, most);
 }
 
 hipError_t launch_mx_dec(int mode, int dtype, const DecArgs& a, hipStream_t stream) {
     if (a.P > kDecMaxPairs || a.E > kDecMaxE || a.ks_lim != 1 || a.meta == nullptr || a.mx0 == nullptr ||
-        (mode == kGateUp && a.mx1 == nullptr) || a.kc < 512 || a.kc % 512 || a.K % 32 || a.N % 32)
+        (mode == kGateUp && a.mx1 == nullptr) || a.K % 32 || a.N % 32)
         return hipErrorInvalidValue;
     if (dtype == kBF16) return launch_dt<kBF16>(mode, a, stream);
     if (dtype == kF16) return launch_dt<kF16>(mode, a, stream);

@@ -57,8 +57,8 @@ static int run_mx(const MxCall& c, hipStream_t s) {
                          "fused_moe_mxfp4: input, weights and output must be 16-byte aligned");
     if ((long long)c.T * c.H * 2 >= lim || P * c.I * 2 >= lim || (long long)c.H * c.I * 2 >= lim)
         return set_error(CANDLE_MOE_ERR_UNSUPPORTED, "fused_moe_mxfp4: operands beyond 2 GiB");
-    if (!aligned(c.gate_s, 4) || !aligned(c.up_s, 4) || (qwen3 && !aligned(c.down_s, 4)))
-        return set_error(CANDLE_MOE_ERR_UNSUPPORTED, "fused_moe_mxfp4: weight scales must be 4-byte aligned");
+    if (!aligned(c.gate_s, 16) || !aligned(c.up_s, 16) || (qwen3 && !aligned(c.down_s, 16)))
+        return set_error(CANDLE_MOE_ERR_UNSUPPORTED, "fused_moe_mxfp4: weight scales must be 16-byte aligned");
     const MxWeights mx = {reinterpret_cast<const uint8_t*>(c.gate_s), reinterpret_cast<const uint8_t*>(c.up_s),
                           reinterpret_cast<const uint8_t*>(c.down_s), reinterpret_cast<const uint8_t*>(c.x_scale)};
     return fused_moe_impl(c.x, c.gate, c.up, c.down, c.rw, c.idx, c.out, c.T, c.H, c.I, c.E, c.k, c.act, c.moe_type,

@@ -397,7 +397,7 @@ int candle_moe_dequantize_mxfp4(const void* codes, const void* scales, int num_e
  * hidden_dim / 32] in input_scale, counted as dtype(value) (exact in bf16).
  * f32 accumulation; the intermediate is rounded to dtype. accumulate != 0:
  * output += result, else output = result. hidden_dim and intermediate_dim
- * multiples of 32; input, codes and output 16-byte aligned, weight scales 4-byte. The workspace is
+ * multiples of 32; input, codes, weight scales and output 16-byte aligned. The workspace is
  * the library's, as fused_moe's (one call of the largest size before capturing
  * serves every smaller one). */
 int candle_moe_fused_moe_mxfp4(const void* input, const void* input_scale, const void* gate_q, const void* up_q,

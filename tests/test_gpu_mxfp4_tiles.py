@@ -77,5 +77,5 @@ def test_an_unaligned_view_of_the_scales_is_refused(policies):
     s = setup(4, 64, 64, 2, 1, 0, BF, False)
     flat = torch.zeros(s["gate"][1].numel() + 1, dtype=torch.uint8, device="cuda")
     s["gate"] = (s["gate"][0], flat[1:].view_as(s["gate"][1]))
-    with pytest.raises(cm.CandleMoeError, match="4-byte aligned"):
+    with pytest.raises(cm.CandleMoeError, match="scales must be 16-byte aligned"):
         run(s, 0, torch.empty(4, 64, dtype=BF, device="cuda"))
