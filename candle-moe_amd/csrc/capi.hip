@@ -607,7 +607,7 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
     p.set_from = 0.0;
     // (fp8 weights: on the 8-wave prefill kernel, whose expert-set GEMM keeps
     // its accumulators in per-segment column units)
-    if (p.mfma && (!fp8 || p.cfg == kLds256w8) && out16 && (I % 64) == 0 && k <= kSetMaxK &&
+    if (p.mfma && (!fp8 || p.cfg == kLds256w8) && out16 && (I % (mx ? 128 : 64)) == 0 && k <= kSetMaxK &&
         g_combine_policy != 1) {
         long long nk = 1;
         for (int j = 0; j < k && nk <= kSetMaxKeys; ++j) nk *= (E + 1);

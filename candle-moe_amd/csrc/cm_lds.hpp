@@ -87,15 +87,17 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // distinct bank groups.
 template <int ACH>
 __device__ __forceinline__ int a_swz(int r, int c) {
-    if constexpr (ACH == 8) return (c ^ r ^ (r >> 3)) & 7;
+    if constexpr (ACH == 16) return (c ^ r) & 15;
+    else if constexpr (ACH == 8) return (c ^ r ^ (r >> 3)) & 7;
     else return (c ^ (r >> 2)) & 3;
 }
 
 // Rows of 4-bit codes (KCH chunks of 32 k): a lane reads one 16-byte chunk of its
-// row; rows 32 bytes apart, so of 16 rows the second eight swap their chunks.
+// row; rows are 32 (64) bytes apart, so of 16 rows the second eight swap their
+// chunks (every four rows take another order of them).
 template <int KCH>
 __device__ __forceinline__ int w4_swz(int r, int c) {
-    return KCH == 2 ? c ^ ((r >> 3) & 1) : c;
+    return KCH == 4 ? (c ^ (r >> 2)) & 3 : KCH == 2 ? c ^ ((r >> 3) & 1) : c;
 }
 
 // [K,N] sub-tile rows of BCH 16-byte chunks: chunk c of k-row r is stored at

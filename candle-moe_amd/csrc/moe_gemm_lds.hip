@@ -79,7 +79,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     constexpr bool ROWS = (MODE == kDownRows || MODE == kFc2Rows);
     constexpr bool ATOMIC = (MODE == kDown || MODE == kFc2);
     constexpr bool SWAP = !ATOMIC;
-    static_assert(BK == 32 || BK == 64, "BK");
+    static_assert(BK == 32 || BK == 64 || (W4 && BK == 128), "BK");
     constexpr int ACH = BK / 8;            // 16-byte chunks per K-contiguous row
     constexpr int AROW = BK * 2;           // bytes per K-contiguous row
     constexpr int RPA = 1024 / AROW;       // K-contiguous rows per DMA instruction
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     constexpr int KCH = KROW / 16;
     constexpr int KRPI = 1024 / KROW;  // n-rows of codes per DMA instruction
     constexpr int B_BYTES = W8 || W4 ? BN * KROW : BN * AROW;
-    constexpr int SDW = BK / 32;       // W4: scale dwords per column and stage
+    constexpr int SDW = BK == 32 ? 1 : 2;  // W4: scale dwords per column and stage
     constexpr int S_BYTES = W4 ? BN * 4 * SDW : 0;
     constexpr int S_INS = S_BYTES / (256 * NW);  // (one dword per lane)
     static_assert(S_INS * 256 * NW == S_BYTES, "scale DMA split");
@@ -100,6 +100,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     constexpr bool EX = EXT > 0;
     constexpr int NX = EX ? NB / 2 : 1;     // column blocks of the extension rows per wave
     constexpr int X_INS = EX ? EXT / RPA : 1;  // DMA instructions of the extension rows (per stage)
+    constexpr int XN = X_INS > NW ? X_INS / NW : 1;  // and per wave
     constexpr int X_OFF = A_BYTES + B_BYTES + S_BYTES;
     constexpr int STAGE = X_OFF + EXT * AROW;
     constexpr int A_INS = A_BYTES / (1024 * NW);  // DMA instructions per wave per stage
@@ -219,18 +220,32 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     // extension rows: instruction wave % X_INS of X_INS (every wave issues
     // one, so that the waves' DMA counts stay equal; repeats write the same
     // bytes)
-    const int x_q = EX ? wave % X_INS : 0;
-    uint32_t x_off = kOob;
+    int x_q[XN];
+    uint32_t x_off[XN];
+#pragma unroll
+    for (int i = 0; i < XN; ++i) {
+        x_q[i] = EX ? (NW * i + wave) % X_INS : 0;
+        x_off[i] = kOob;
+    }
+    auto x_chunk = [&](int i) { return a_swz<ACH>(RPA * x_q[i] + lane / ACH, lane % ACH) * 8; };  // its first k
     auto set_x_off = [&]() {
-        const int xr = RPA * x_q + lane / ACH;  // row of the block
-        const int r = BM + xr;
-        const int kc = a_swz<ACH>(xr, lane % ACH) * 8;
-        if constexpr (GATHER) {
-            const int src = a.sorted_pair[min(r0 + r, a.sorted_n - 1)] / a.k_top;
-            x_off = ((uint32_t)src * (uint32_t)a_pitch + (uint32_t)kc) * 2u;
-        } else {
-            x_off = r < m_valid ? ((uint32_t)(r0 + r) * (uint32_t)a_pitch + (uint32_t)kc) * 2u : kOob;
+#pragma unroll
+        for (int i = 0; i < XN; ++i) {
+            const int r = BM + RPA * x_q[i] + lane / ACH;
+            const int kc = x_chunk(i);
+            if constexpr (GATHER) {
+                const int src = a.sorted_pair[min(r0 + r, a.sorted_n - 1)] / a.k_top;
+                x_off[i] = ((uint32_t)src * (uint32_t)a_pitch + (uint32_t)kc) * 2u;
+            } else {
+                x_off[i] = r < m_valid ? ((uint32_t)(r0 + r) * (uint32_t)a_pitch + (uint32_t)kc) * 2u : kOob;
+            }
         }
+    };
+    // all in range, or each lane's chunk checked against K
+    auto issue_x = [&](uint32_t at, int k0, bool whole) {
+#pragma unroll
+        for (int i = 0; i < XN; ++i)
+            dma16s(rA, at + X_OFF + x_q[i] * 1024, whole || k0 + x_chunk(i) < K ? x_off[i] : kOob, (uint32_t)k0 * 2u);
     };
     // B [N,K]: like A over the column tile's rows n. B [K,N]: instruction i
     // (i % SUB_INS within sub-tile i / SUB_INS) covers k-rows RPI*q ..
@@ -367,14 +382,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
                 }
             }
             if constexpr (EX) {
-                if (xrows) dma16s(rA, sA + X_OFF + x_q * 1024, x_off, sa);
+                if (xrows) issue_x(sA, k0, true);
             }
         } else {
             if constexpr (EX) {
-                if (xrows) {
-                    const bool in = k0 + a_swz<ACH>(RPA * x_q + lane / ACH, lane % ACH) * 8 < K;
-                    dma16s(rA, sA + X_OFF + x_q * 1024, in ? x_off : kOob, sa);
-                }
+                if (xrows) issue_x(sA, k0, false);
             }
             // K tail: every lane's chunk is checked against the operand's K
 #pragma unroll
@@ -432,8 +444,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     // share of it follows
     auto issue_first_x = [&](int k0) {
         set_x_off();
-        const bool in = k0 + BK <= K || k0 + a_swz<ACH>(RPA * x_q + lane / ACH, lane % ACH) * 8 < K;
-        dma16s(rA, smem_base + X_OFF + x_q * 1024, in ? x_off : kOob, (uint32_t)k0 * 2u);
+        issue_x(smem_base, k0, k0 + BK <= K);
     };
 
     f32x16 acc[MB][NB];
@@ -730,7 +741,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
         const char* sS = sB + B_BYTES;
         u32x4 af[2][MB], bfr[NB], xf;
         uint32_t braw[NB][KSTEPS];
-        float sc[NB];
+        constexpr int GRP = BK == 128 ? 2 : 1;  // scales per lane and column
+        float sc[NB][GRP];
         auto load_a = [&](int kk) {
             const int c = lh * KSTEPS + kk;
 #pragma unroll
@@ -744,21 +756,25 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
         for (int nb = 0; nb < NB; ++nb) {
             const int r = (DUAL ? (nb & 1) * SUBN + wn * (WN / 2) + (nb >> 1) * 32 : wn * WN + nb * 32) + lr;
             const uint32_t first = (uint32_t)(nt * SUBN + r % SUBN) * (uint32_t)(a.ldb / 32) + (uint32_t)(kk0 / 32);
-            if constexpr (BK == 64) {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(sB + r * KROW + w4_swz<KCH>(r, lh) * 16);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) braw[nb][q % KSTEPS] = v[q];
+            if constexpr (BK >= 64) {
                 const uint64_t d = *reinterpret_cast<const uint64_t*>(sS + r * 8);
-                uint32_t e = (uint32_t)(d >> (8u * ((first & 3u) + (uint32_t)lh))) & 255u;
-                // (past K: the codes are zeros, a foreign scale could be a NaN)
-                if (kk0 + 32 * lh >= klim) e = 127u;
-                sc[nb] = __uint_as_float(e << 23);
+#pragma unroll
+                for (int h = 0; h < GRP; ++h) {
+                    const int gr = GRP * lh + h;  // 32 k of the tile
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(sB + r * KROW + w4_swz<KCH>(r, gr) * 16);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) braw[nb][(4 * h + q) % KSTEPS] = v[q];
+                    uint32_t e = (uint32_t)(d >> (8u * ((first & 3u) + (uint32_t)gr))) & 255u;
+                    // (past K: the codes are zeros, a foreign scale could be a NaN)
+                    if (kk0 + 32 * gr >= klim) e = 127u;
+                    sc[nb][h] = __uint_as_float(e << 23);
+                }
             } else {
                 const u32x2 v = *reinterpret_cast<const u32x2*>(sB + r * KROW + lh * 8);
                 braw[nb][0] = v[0];
                 braw[nb][KSTEPS - 1] = v[1];
                 const uint32_t d = *reinterpret_cast<const uint32_t*>(sS + r * 4);
-                sc[nb] = __uint_as_float(((d >> (8u * (first & 3u))) & 255u) << 23);
+                sc[nb][0] = __uint_as_float(((d >> (8u * (first & 3u))) & 255u) << 23);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -767,7 +783,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
             if (kk + 1 < KSTEPS) load_a(kk + 1);
             if constexpr (X) load_x(sA, kk, xf);
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) bfr[nb] = mx4x8_to<DT>(braw[nb][kk], sc[nb]);
+            for (int nb = 0; nb < NB; ++nb) bfr[nb] = mx4x8_to<DT>(braw[nb][kk], sc[nb][kk / 4 % GRP]);
             mfma_step(af[kk & 1], bfr);
             if constexpr (X) mfma_x(xf, bfr);
             if (kk + 1 < KSTEPS) interleave(x);
@@ -849,7 +865,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
         constexpr bool X = decltype(x)::value;
         // wait for the DMA of the tile with `newer` of this wave's tiles
         // issued after it
-        auto wait_tile = [&](int newer) { wait_stage<LOADS + (X ? 1 : 0), NST - 2>(newer); };
+        auto wait_tile = [&](int newer) { wait_stage<LOADS + (X ? XN : 0), NST - 2>(newer); };
         u32x4 af0[MB], bf0[NB], af1[MB], bf1[NB], xf;
         auto mfmas = [&](const u32x4 (&af)[MB], const u32x4 (&bf)[NB], const char* sA, int kk) {
             if constexpr (X) load_x(sA, kk, xf);
@@ -927,7 +943,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     if constexpr (X) stage_x_rows();
     for (int kt = 0; kt < nk; ++kt) {
         const int newer = min(NST - 2, nk - 1 - kt);  // stages issued after kt and before this wait
-        wait_stage<LOADS + (X ? 1 : 0), NST - 2>(newer);
+        wait_stage<LOADS + (X ? XN : 0), NST - 2>(newer);
         wait_lgkm0();
         block_barrier();
         const int ahead = kt + NST - 1;
@@ -1136,7 +1152,7 @@ static hipError_t launch_mx_mode(int cfg, const GemmArgs& a, hipStream_t stream)
     constexpr int X = kTileExt;
     switch (cfg) {
         case kLds128:
-            hipLaunchKernelGGL((moe_lds_gemm<DT, 128, 128, 64, 4, 4, MODE, 2, 1, false, false, X, true>), g, dim3(256), 0,
+            hipLaunchKernelGGL((moe_lds_gemm<DT, 128, 128, 128, 3, 4, MODE, 2, 1, false, false, X, true>), g, dim3(256), 0,
                                stream, a);
             break;
         case kLds256w8:
@@ -1151,12 +1167,12 @@ static hipError_t launch_mx_mode(int cfg, const GemmArgs& a, hipStream_t stream)
             if constexpr (MODE != kDownSet) {
                 if constexpr (MODE != kGateUp) {
                     if (a.narrow) {
-                        hipLaunchKernelGGL((moe_lds_gemm<DT, 32, 128, 64, 4, 4, MODE, 1, 1, false, false, 0, true>), g,
+                        hipLaunchKernelGGL((moe_lds_gemm<DT, 32, 128, 128, 4, 4, MODE, 1, 1, false, false, 0, true>), g,
                                            dim3(256), 0, stream, a);
                         break;
                     }
                 }
-                hipLaunchKernelGGL((moe_lds_gemm<DT, 32, 256, 64, 4, 4, MODE, 1, 1, false, false, 0, true>), g, dim3(256),
+                hipLaunchKernelGGL((moe_lds_gemm<DT, 32, 256, 128, 4, 4, MODE, 1, 1, false, false, 0, true>), g, dim3(256),
                                    0, stream, a);
                 break;
             }
