@@ -527,12 +527,12 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
         // 51 / 78 / 73, T=2000 73 / 71 / 90 / 87).
         const long long stream = est_tiles(32) * (p.moe_type == kQwen3 ? 3LL : 2LL) * H * I * 17 / 32;
         p.cfg = P <= kMxDecPairs && dec_gemv_fits(p) ? kDecGemv
-                : P <= 32 * touched || (P <= 256 * touched && stream <= kMxRows32StreamBytes) ? kLdsRows32
+                : P <= 32 * touched || (P <= 384 * touched && stream <= kMxRows32StreamBytes) ? kLdsRows32
                                                                                             : kLds256w8;
         const int mode1 = p.moe_type == kQwen3 ? kGateUp : kFc1;
         const long long dev_wgs = 8LL * std::max(cus_per_xcd(), 32);
         if (p.cfg == kLds256w8 && P <= kOneTileRows * touched)
-            p.cfg = 2 * touched * cdiv(I, gemm_tile_cols(mode1, kLds128)) <= 3 * dev_wgs ? kLds128 : kLds128x256o2;
+            p.cfg = touched * cdiv(I, gemm_tile_cols(mode1, kLds128)) <= 2 * dev_wgs ? kLds128 : kLds128x256o2;
         else if (p.cfg == kLds256w8 && H <= 1024 && est_tiles(256) * cdiv(I, gemm_tile_cols(mode1, kLds256w8)) < dev_wgs)
             p.cfg = kLds128;
         if ((is_lds_cfg(g_tile_policy) && g_tile_policy != kW8Gemv) || (g_tile_policy == kDecGemv && dec_gemv_fits(p)))

@@ -134,7 +134,8 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     // staged (row-contiguous) epilogue of the large tiles, see staged_epilogue
     constexpr bool R32 = W4 && ROWS;  // f32 pair rows, unweighted (summed with the weights afterwards)
     constexpr bool STAGED = SWAP && BM >= 128 && !R32;
-    constexpr int OUT_BYTES = STAGED ? BM * (DUAL ? BN / 2 : BN) * 2 : 0;
+    constexpr bool STAGED32 = R32 && BM >= 128;  // (in f32, half of the columns at a time)
+    constexpr int OUT_BYTES = STAGED ? BM * (DUAL ? BN / 2 : BN) * 2 : STAGED32 ? BM * (BN / 2) * 4 : 0;
     static_assert(!STAGED || W4 || NST * STAGE >= OUT_BYTES, "output tile fits the stages");
     constexpr int SMEM = NST * STAGE > OUT_BYTES ? NST * STAGE : OUT_BYTES;
     __shared__ __attribute__((aligned(1024))) char smem[SMEM];
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     // column scale, or 1 for an all-zero column), [kSetMaxK][BN]
     constexpr bool W8SET = W8 && SET;
     __shared__ __attribute__((aligned(16))) float s_unit[W8SET ? kSetMaxK * BN : 4];
-    __shared__ int32_t s_dst[STAGED || (R32 && EX) ? BM + EXT : 1];
+    __shared__ int32_t s_dst[STAGED || STAGED32 ? BM + EXT : 1];
     __shared__ float s_wx[EX ? EXT : 1];  // routing weights of the extension rows
 
     // workgroup -> (output tile, K split); every workgroup first clears its
@@ -1014,10 +1015,18 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     }
     const int m_tile = EX ? min(m_valid, BM) : m_valid;  // the tile's own rows
     if constexpr (R32) {
-        rows32_epilogue<BN, WM, WN, MB, NB>(a, acc, m_tile, nt, wm, wn, lane, pre_dst);
+        if constexpr (STAGED32) {
+            if (wn == 0 && lane < 32) {
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb) s_dst[wm * WM + mb * 32 + lane] = pre_dst[mb];
+            }
+            __syncthreads();  // every wave is done with the stages
+            staged_rows32<BM, BN, WM, WN, MB, NB, NW>(a, acc, smem, s_dst, m_tile, nt, wm, wn, lane);
+        } else {
+            rows32_epilogue<BN, WM, WN, MB, NB>(a, acc, m_tile, nt, wm, wn, lane, pre_dst);
+        }
         if constexpr (EX) {
             if (ext_rows) {
-                __syncthreads();  // (stage_x_rows ran on one wave)
                 f32x16 blk[1][NX];
 #pragma unroll
                 for (int j = 0; j < NX; ++j) blk[0][j] = accx[j];
