@@ -1010,7 +1010,10 @@ static int run_moe(const Problem& p, const void* x, const void* gate, const void
         pair_dest = reinterpret_cast<int32_t*>(ws + L.pair_dest);
     }
     if (p.cfg == kDecGemv) return run_moe_dec(p, x, gate, up, down, rw, idx, out, overwrite, ws, L, s, f8, mx);
-    if (mx && mx->x_s) {
+    // (bf16, which holds every MX value: in f16 the values count as rounded to it)
+    const bool native8 = mx && mx->x_s && p.cfg == kLds256w8 && p.dtype == kBF16 && p.H % 128 == 0 &&
+                         ((uintptr_t)mx->x_s & 3) == 0;
+    if (mx && mx->x_s && !native8) {
         // MXFP8 rows in 16 bits, exactly (bf16): the tile kernels' operand
         ProfScope ps(kSlotGroup, s);
         e = launch_rows8_to(x, mx->x_s, p.T, p.H, ws + L.rows16, p.dtype, s);
@@ -1081,10 +1084,14 @@ static int run_moe(const Problem& p, const void* x, const void* gate, const void
         g1.ldb = p.H;
         g1.mx0 = mx->gate_s;
         g1.mx1 = mx->up_s;
+        if (native8) {
+            g1.xs = mx->x_s;
+            g1.a_bytes = (long long)p.T * p.H;
+        }
     }
     {
         ProfScope ps(kSlotGemm1, s);
-        e = gemm(mode1, g1);
+        e = native8 ? launch_moe_gemm_mx8(mode1, g1, s) : gemm(mode1, g1);
     }
     if (e != hipSuccess) return hip_fail(e, "fused_moe gate/up GEMM");
 

@@ -173,6 +173,8 @@ struct GemmArgs {
     // (kGateUp) B1, 4-byte aligned; codes [E][N][K/2], strideB = N * K, ldb = K
     const uint8_t* mx0;
     const uint8_t* mx1;
+    // launch_moe_gemm_mx8: A is MXFP8 codes (a_bytes = T * K), their scale bytes
+    const uint8_t* xs;
     // 32-row kernel, kFc1 / kDown / kFc2 with 16-bit weights: 128-column
     // tiles instead of 256 (n_tiles counts those)
     int narrow;
@@ -308,6 +310,9 @@ hipError_t launch_moe_gemm_w8(int mode, int dtype, int cfg, const GemmArgs& a, h
 // [T*k, N] by pair, unweighted), kDownSet / kFc2Set; cfg kLdsRows32 (not the
 // sets), kLds128, kLds128x256o2 or kLds256w8
 hipError_t launch_moe_gemm_mx(int mode, int dtype, int cfg, const GemmArgs& a, hipStream_t stream);
+// kGateUp and kFc1 over MXFP4 weights and MXFP8 rows, both as they are, on the
+// 256x256 tile table, bf16 out (K a multiple of 128, xs 4-byte aligned)
+hipError_t launch_moe_gemm_mx8(int mode, const GemmArgs& a, hipStream_t stream);
 // kW8Gemv (moe_gemv_w8.hip): modes kGateUp, kFc1, kDown, kFc2 (pair path,
 // f32 atomics for kDown / kFc2)
 hipError_t launch_w8_gemv(int mode, int dtype, const GemmArgs& a, hipStream_t stream);

@@ -232,7 +232,7 @@ struct RouteFast {
 // WHOLE: every lane holds VPT experts or none, and logits and biases are read 16
 // bytes at a time.
 template <int LPR, int VPT, int DT, bool WHOLE>
-__global__ __launch_bounds__(64 * kRouteWaves) void route_fast_k(RouteArgs a, RouteFast f) {
+__global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void route_fast_k(RouteArgs a, RouteFast f) {
     typedef typename Elem<DT>::storage S;
     constexpr int RPW = 64 / LPR, SLOTS = LPR * VPT, VS = SLOTS > 64 ? SLOTS / 64 : 1;
     constexpr int IB = SLOTS == 64 ? 6 : SLOTS == 128 ? 7 : SLOTS == 256 ? 8 : SLOTS == 512 ? 9 : 10;

@@ -98,11 +98,13 @@ def act64(x, act):
     return torch.relu(x)
 
 
-def moe(x, gate, up, down, rw, idx, act, moe_type, dtype, rounded=True):
+def moe(x, gate, up, down, rw, idx, act, moe_type, dtype, rounded=True, aligned=0.0):
     """The MoE in 64 bits over weights [E, N, K], and how far a result of `dtype`
     may be from it: the intermediate, each pair's row and the output rounded to
     dtype once (half a step each), f32 sums (2^-24 per term and rounding), the
-    activation within 2^-20 (its slope is at most 1.13)."""
+    activation within 2^-20 (its slope is at most 1.13). aligned: of the first
+    products' sum of magnitudes, what their sums may lose (8-bit rows on the scaled
+    matrix instruction, which aligns 64 terms to the largest: 64 * 2^-18 of it)."""
     T, H = x.shape
     E = gate.shape[0]
     u, tiny = HALF[dtype], LEAST[dtype]
@@ -113,11 +115,11 @@ def moe(x, gate, up, down, rw, idx, act, moe_type, dtype, rounded=True):
         if not t.numel():
             continue
         a, g = x[t].double(), gate[e].t()
-        s, ds = a @ g, (a.abs() @ g.abs()) * (a.shape[1] + 4) * 2.0 ** -24
+        s, ds = a @ g, (a.abs() @ g.abs()) * ((a.shape[1] + 4) * 2.0 ** -24 + aligned)
         h, dh = act64(s, act), 1.13 * ds + 2.0 ** -20 * act64(s, act).abs() + 2.0 ** -126
         last = up[e].t()
         if moe_type == 0:
-            v, dv = a @ last, (a.abs() @ last.abs()) * (a.shape[1] + 4) * 2.0 ** -24
+            v, dv = a @ last, (a.abs() @ last.abs()) * ((a.shape[1] + 4) * 2.0 ** -24 + aligned)
             dh = dh * (v.abs() + dv) + h.abs() * dv
             h = h * v
             last = down[e].t()

@@ -92,16 +92,16 @@ def run(s, act, out, accumulate=False):
     return out
 
 
-def want(s, act):
+def want(s, act, aligned=0.0):
     x = s["x"] if s["x_scale"] is None else ref.from_mxfp8(s["x"], s["x_scale"])
     w = [ref.from_mxfp4(*q) if q[0] is not None else None for q in (s["gate"], s["up"], s["down"])]
-    return ref.moe(x, *w, s["rw"], s["idx"], act, s["moe_type"], s["dtype"])
+    return ref.moe(x, *w, s["rw"], s["idx"], act, s["moe_type"], s["dtype"], aligned=aligned)
 
 
-def check(s, act, what=""):
+def check(s, act, what="", aligned=0.0):
     T, H = s["x"].shape
     out = torch.full((T, H), float("nan"), dtype=s["dtype"], device="cuda")
-    ref.within(run(s, act, out), *want(s, act), what)
+    ref.within(run(s, act, out), *want(s, act, aligned), what)
     return out
 
 

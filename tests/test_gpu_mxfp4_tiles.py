@@ -52,6 +52,33 @@ def test_long_k_in_splits(tile, policies):
     check(setup(300, 2080, 4128, 2, 1, 1, BF, False, seed=5), 1)
 
 
+@pytest.mark.parametrize("sets", [False, True])
+@pytest.mark.parametrize("moe_type", [0, 1])
+@pytest.mark.parametrize("T, H, I, E, k", [(1, 128, 32, 1, 1), (130, 256, 160, 2, 2), (257, 384, 288, 1, 1), (300, 128, 544, 5, 3),
+                                          (600, 1152, 256, 2, 1), (700, 4224, 128, 4, 2)])
+def test_eight_bit_rows_as_they_are(T, H, I, E, k, moe_type, sets, policies):
+    # the gate/up and fc1 products in the MX formats themselves (256x256 tiles)
+    cm.set_tile_policy(cm.TILE_W8)
+    cm.set_combine_policy(cm.COMBINE_EXPERT_SETS if sets else cm.COMBINE_PAIRS)
+    s = setup(T, H, I, E, k, moe_type, BF, True, seed=T, dropped=0.1)
+    first = check(s, T % 3, aligned=2.0 ** -12)
+    assert torch.equal(first, check(s, T % 3, aligned=2.0 ** -12))
+
+
+def test_eight_bit_rows_with_scales_far_apart(policies):
+    cm.set_tile_policy(cm.TILE_W8)
+    s = setup(40, 512, 128, 2, 1, 0, BF, True, seed=11)
+    for q in (s["x_scale"], s["gate"][1], s["up"][1]):
+        q.copy_((120 + (torch.arange(q.numel(), device="cuda") * 7) % 11).to(torch.uint8).view_as(q))
+    s["x_scale"][3] = 0
+    check(s, 2, aligned=2.0 ** -12)
+    s["gate"][1][1, 5] = 255
+    hit = (s["idx"] == 1).any(1)
+    # (SiLU: the ReLU, max(x, 0), takes a NaN to 0 as everywhere here)
+    out = run(s, 0, torch.empty(40, 512, dtype=BF, device="cuda"))
+    assert torch.isnan(out[hit]).all() and not torch.isnan(out[~hit]).any()
+
+
 @pytest.mark.parametrize("tile", TILES)
 def test_foreign_scales_do_not_reach_the_columns_of_an_expert(tile, policies):
     # K = 3 * 32: the half tile past the end of a row lies before the next row's
