@@ -520,11 +520,15 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
         // expert's codes once per 32 rows, up to 32 rows per touched expert or
         // while that stream stays within kMxRows32StreamBytes; then, as for 16-bit
         // weights, 128-row tiles while an expert's rows fit one, 128x128 where
-        // they are few or the 256x256 tiles number less than the CUs (steps, 32-row / 128x128 / 128x256 / 256x256 tiles: Qwen3
-        // T=256 73 / 79 / 127 / 97 us, T=500 115 / 90 / 145 / 123, T=1024 207 / 159
-        // / 150 / 157, T=2048 - / 294 / 283 / 223; Qwen3-30B-A3B T=1024 229 / 260 /
-        // 209 / 220, T=2048 369 / 322 / 281 / 289; H 768 I 2048 E 8 k 2 T=777 45 /
-        // 51 / 78 / 73, T=2000 73 / 71 / 90 / 87).
+        // they are few or the 256x256 tiles number less than the CUs (steps,
+        // 32-row / 128x128 / 128x256 / 256x256 tiles: Qwen3 T=256 66 / 68 / 127 /
+        // 97 us, T=500 106 / 85 / 144 / 120, T=1024 207 / 159 / 150 / 157, T=2048
+        // - / 294 / 283 / 223; Qwen3-30B-A3B T=1024 229 / 260 / 209 / 220, T=2048
+        // 369 / 322 / 281 / 289; H 768 I 2048 E 8 k 2 T=777 44 / 46 / 79 / 71,
+        // T=2000 73 / 71 / 90 / 87). Long rows of few experts also leave the
+        // 32-row kernel where its tiles pass one round of the CUs and the 128x128
+        // tiles do not (Qwen3 T=280 81 against 69 us, T=320 88 against 69; with H
+        // 768 the 32-row kernel stays ahead, T=500 40 against 51).
         const long long stream = est_tiles(32) * (p.moe_type == kQwen3 ? 3LL : 2LL) * H * I * 17 / 32;
         p.cfg = P <= kMxDecPairs && dec_gemv_fits(p) ? kDecGemv
                 : P <= 32 * touched || (P <= 384 * touched && stream <= kMxRows32StreamBytes) ? kLdsRows32
@@ -535,6 +539,13 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
             p.cfg = touched * cdiv(I, gemm_tile_cols(mode1, kLds128)) <= 2 * dev_wgs ? kLds128 : kLds128x256o2;
         else if (p.cfg == kLds256w8 && H <= 1024 && est_tiles(256) * cdiv(I, gemm_tile_cols(mode1, kLds256w8)) < dev_wgs)
             p.cfg = kLds128;
+        if (p.cfg == kLdsRows32 && H > 1024 && P > 32 * touched &&
+            (est_tiles(32) + touched / 2) * cdiv(I, gemm_tile_cols(mode1, kLdsRows32)) > dev_wgs &&
+            touched * cdiv(I, gemm_tile_cols(mode1, kLds128)) <= dev_wgs && P <= kOneTileRows * touched)
+            p.cfg = kLds128;
+        // 8-bit rows that go as they are (bf16): the 256x256 kernel has that form
+        // (Qwen3-30B-A3B T=1024 / 2048 181 / 224 us against 210 / 278)
+        if (p.cfg == kLds128x256o2 && mx8 && p.dtype == kBF16 && H % 128 == 0) p.cfg = kLds256w8;
         if ((is_lds_cfg(g_tile_policy) && g_tile_policy != kW8Gemv) || (g_tile_policy == kDecGemv && dec_gemv_fits(p)))
             p.cfg = g_tile_policy;
     } else if (p.mfma && !policy) {
@@ -667,7 +678,8 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
     // loads in flight lost 2.6-3.5 us at Qwen3 T=16 / 64.) fp8 weights the
     // same: Nomic T=16 fc1 17.6 -> 12.5 us, against 14.5 us with bf16 weights)
     const long long dev_wgs = 8LL * std::max(cus_per_xcd(), 32);
-    p.narrow1 = p.cfg == kLdsRows32 && p.moe_type == kNomic && touched * cdiv(I, 256) < dev_wgs;
+    p.narrow1 = p.cfg == kLdsRows32 && p.moe_type == kNomic &&
+                (mx ? est_tiles(32) : touched) * cdiv(I, 256) < dev_wgs;
     if (p.narrow1) p.n_tiles1 = cdiv(I, 128);
     // Decode down / fc2 GEMM (32-row kernel, 16-bit weights): 128-column
     // tiles where the 256-column tiling would leave CUs without a tile (and
@@ -678,7 +690,7 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
     // tiles enough for every CU the wide tiles stay ahead (T=1: 13.1 against
     // 13.6 us, T=16: 50.6 against 56.1 us). fp8 weights the same: Qwen3 T=16
     // / 64 20.4 -> 16.2, 20.5 -> 16.6 us.
-    const int down_cols = (p.cfg == kLdsRows32 && I >= 1536 && touched * cdiv(H, 256) < dev_wgs)
+    const int down_cols = (p.cfg == kLdsRows32 && I >= 1536 && (mx ? est_tiles(32) : touched) * cdiv(H, 256) < dev_wgs)
                               ? 128
                               : gemm_tile_cols(kDown, p.cfg);
     p.narrow2 = down_cols == 128 && gemm_tile_cols(kDown, p.cfg) != 128;
