@@ -806,7 +806,7 @@ static size_t upto_bytes(const Problem& p) {
                 if (p.set_path && g_combine_policy == 0) t = std::min(t, std::ceil(p.set_from));
                 acc = std::max(acc, (size_t)std::min(t * p.k * p.H * 2.0, kRowsMaxBytes));
             }
-            if (forced || P > (p.fp8 ? 32 : kOneTileRows) * touched) {
+            if (forced || P > (p.fp8 || p.mx8 ? 32 : kOneTileRows) * touched) {
                 const size_t slots = 8 * (size_t)cus_per_xcd();
                 partial = std::max(partial, slots * 256 * tile_cols(kLds256w8) * 4);
                 o += a256(slots * 4);

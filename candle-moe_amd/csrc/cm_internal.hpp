@@ -31,6 +31,7 @@ hipError_t launch_router_exp_check(uint32_t first, uint32_t n, uint32_t* stats, 
 // kRouteSigmoid; idx, w and ei [T, k].
 enum RouteScore : int { kRouteSoftmax = 0, kRouteSigmoid = 1 };
 constexpr int kRouteMaxGroups = 64;
+constexpr int kRouteMaxRows = 1 << 25;  // (a launch holds fewer than 2^32 threads: 64 per row)
 struct RouteArgs {
     const void* logits;
     const float* bias;  // [E] or null
@@ -57,6 +58,7 @@ struct NormArgs {
     int T, H, vec;
     float eps;
 };
+constexpr int kNormMaxRows = 1 << 21;  // of one launch (up to 1024 threads per row)
 hipError_t launch_add_rms_norm(const NormArgs& a, int dtype, hipStream_t stream);
 
 // -------------------------------------------------------------- grouping

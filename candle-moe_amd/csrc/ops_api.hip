@@ -98,6 +98,10 @@ int candle_moe_topk_route(const void* logits, uint32_t logits_dtype, const float
         return cm::set_error(CANDLE_MOE_ERR_INVALID,
                              "topk_route: topk must be in [1, %d], the experts of the chosen groups (got %d)",
                              topk_groups * (E / G), topk);
+    if ((long long)T * topk > 0x7fffffffLL || T > cm::kRouteMaxRows)
+        return cm::set_error(CANDLE_MOE_ERR_INVALID,
+                             "topk_route: at most %d tokens and 2^31-1 pairs of them and their experts (got %d x %d)",
+                             cm::kRouteMaxRows, T, topk);
     if (T == 0) return CANDLE_MOE_OK;
     if (!logits || !topk_weight || !topk_indices || !token_expert_indices)
         return cm::set_error(CANDLE_MOE_ERR_INVALID, "topk_route: null tensor pointer");
@@ -155,7 +159,24 @@ int candle_moe_add_rms_norm(const void* input, const void* residual, const void*
             cm::aligned(residual_output, 16) && cm::aligned(output, 16) && cm::aligned(codes, 8);
     if (codes && !a.vec)
         return cm::set_error(CANDLE_MOE_ERR_UNSUPPORTED, "add_rms_norm: the 8-bit form needs 16-byte aligned tensors");
-    const hipError_t e = cm::launch_add_rms_norm(a, (int)dtype, reinterpret_cast<hipStream_t>(stream));
+    hipError_t e = hipSuccess;
+    const long long es = dtype == 2 ? 4 : 2;
+    for (long long t = 0; t < T && e == hipSuccess; t += cm::kNormMaxRows) {
+        cm::NormArgs b = a;
+        auto from = [&](const void* p, long long row) {
+            return p ? reinterpret_cast<const char*>(p) + t * row : nullptr;
+        };
+        b.x = from(a.x, H * es);
+        b.residual = from(a.residual, H * es);
+        b.residual_out = const_cast<char*>(from(a.residual_out, H * es));
+        b.out = const_cast<char*>(from(a.out, H * es));
+        if (codes) {
+            b.codes = a.codes + t * H;
+            b.scales = a.scales + t * (H / 32);
+        }
+        b.T = (int)std::min<long long>(T - t, cm::kNormMaxRows);
+        e = cm::launch_add_rms_norm(b, (int)dtype, reinterpret_cast<hipStream_t>(stream));
+    }
     return e == hipSuccess ? CANDLE_MOE_OK : cm::hip_fail(e, "add_rms_norm launch");
 }
 

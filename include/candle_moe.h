@@ -350,7 +350,8 @@ int candle_moe_fused_moe_fp8(const void* input, const void* gate_q, const void* 
  *   logits [num_tokens, num_experts] of logits_dtype, 1 <= num_experts <= 1024;
  *   topk_weight f32, topk_indices u32, token_expert_indices u32 = j * num_tokens +
  *   t, [num_tokens, topk] each, as topk_softmax's; topk at most the
- *   topk_groups * num_experts / num_groups experts of the chosen groups. */
+ *   topk_groups * num_experts / num_groups experts of the chosen groups; at most
+ *   2^25 tokens and 2^31-1 pairs. */
 int candle_moe_topk_route(const void* logits, uint32_t logits_dtype, const float* bias, float* topk_weight,
                           void* topk_indices, void* token_expert_indices, int num_experts, int num_tokens, int topk,
                           int score, int num_groups, int topk_groups, int group_top, int renormalize, float scale,
@@ -395,11 +396,20 @@ int candle_moe_dequantize_mxfp4(const void* codes, const void* scales, int num_e
  * input [num_tokens, hidden_dim] of dtype (f16, bf16) with input_scale NULL, or
  * the MXFP8 codes of candle_moe_add_rms_norm with their scales [num_tokens,
  * hidden_dim / 32] in input_scale, counted as dtype(value) (exact in bf16).
- * f32 accumulation; the intermediate is rounded to dtype. accumulate != 0:
- * output += result, else output = result. hidden_dim and intermediate_dim
- * multiples of 32; input, codes, weight scales and output 16-byte aligned. The workspace is
- * the library's, as fused_moe's (one call of the largest size before capturing
- * serves every smaller one). */
+ * f32 accumulation; the intermediate is rounded to dtype, a token's rows of its
+ * experts are summed unrounded, in slot order. On the 256x256 kernel bf16 calls
+ * whose hidden_dim is a multiple of 128 multiply 8-bit rows as they are: the
+ * matrix instruction then aligns the 64 products of a step to the largest, up to
+ * 2^-12 of the sum of their magnitudes off (2^-16 typically), which rows and
+ * weights of like sizes do not show. accumulate != 0: output += result, else
+ * output = result. hidden_dim and intermediate_dim multiples of 32; input, codes,
+ * weight scales and output 16-byte aligned (input_scale anywhere, 4-byte aligned
+ * for the products as they are). The workspace is the library's, as fused_moe's
+ * (one call of the largest size before capturing serves every smaller one).
+ * Kernels (candle_moe_set_tile_policy 18, 12, 5, 14, 7): decode up to 128 pairs,
+ * 32-row tiles while an expert has at most 32 rows or the streamed codes stay
+ * within 192 MiB, then 128x128 and 128x256 tiles while its rows fit one, else
+ * 256x256. */
 int candle_moe_fused_moe_mxfp4(const void* input, const void* input_scale, const void* gate_q, const void* up_q,
                                const void* down_q, const void* gate_scale, const void* up_scale, const void* down_scale,
                                const void* routing_weights, const void* expert_indices, void* output, int num_tokens,
