@@ -520,31 +520,43 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
         // expert's codes once per 32 rows, up to 32 rows per touched expert or
         // while that stream stays within kMxRows32StreamBytes; then, as for 16-bit
         // weights, 128-row tiles while an expert's rows fit one, 128x128 where
-        // they are few or the 256x256 tiles number less than the CUs (steps,
-        // 32-row / 128x128 / 128x256 / 256x256 tiles: Qwen3 T=256 66 / 68 / 127 /
-        // 97 us, T=500 106 / 85 / 144 / 120, T=1024 207 / 159 / 150 / 157, T=2048
-        // - / 294 / 283 / 223; Qwen3-30B-A3B T=1024 229 / 260 / 209 / 220, T=2048
-        // 369 / 322 / 281 / 289; H 768 I 2048 E 8 k 2 T=777 44 / 46 / 79 / 71,
-        // T=2000 73 / 71 / 90 / 87). Long rows of few experts also leave the
-        // 32-row kernel where its tiles pass one round of the CUs and the 128x128
-        // tiles do not (Qwen3 T=280 81 against 69 us, T=320 88 against 69; with H
-        // 768 the 32-row kernel stays ahead, T=500 40 against 51).
+        // they are few (steps, 32-row / 128x128 / 128x256 / 256x256 tiles: Qwen3
+        // T=256 66 / 68 / 127 / 96 us, T=500 106 / 85 / 174 / 121; Qwen3-30B-A3B
+        // T=512 152 / 219 / 164 / 209, T=1024 228 / 231 / 186 / 224). Long rows of
+        // few experts also leave the 32-row kernel where its tiles pass one round
+        // of the CUs and the 128x128 tiles do not (Qwen3 T=280 81 against 69 us,
+        // T=320 88 against 69; with H 768 the 32-row kernel stays ahead, T=500 40
+        // against 51).
+        // Larger groups: 256x256 tiles (128x128 / 128x256 / 256x256 tiles: Qwen3 T=1024
+        // 144 / 178 / 153 us, T=4096 470 / 408 / 371; Qwen3-30B-A3B T=3000 461 /
+        // 357 / 339, T=8192 1008 / 813 / 827, T=16384 1967 / 1544 / 1495). Groups
+        // about one such tile long, half of them with a second, almost empty one,
+        // are ahead on 128x256 tiles (their extended tiles hold up to 288 rows in
+        // two), where those fill two workgroups of every CU: Qwen3-30B-A3B T=4096
+        // 447 against 482 us, H 2880 I 1024 E 32 k 4 T=2000 222 against 243 (T=3000,
+        // 375 rows: 315 against 274). Short rows (H <= 1024) take the smallest
+        // tiles that fill the device (H 768 I 2048 E 8 k 2: T=2000 67 / 85 / 84,
+        // T=3000 99 / 89 / 90, T=4096 116 / 105 / 121, T=8192 203 / 162 / 164).
         const long long stream = est_tiles(32) * (p.moe_type == kQwen3 ? 3LL : 2LL) * H * I * 17 / 32;
         p.cfg = P <= kMxDecPairs && dec_gemv_fits(p) ? kDecGemv
                 : P <= 32 * touched || (P <= 384 * touched && stream <= kMxRows32StreamBytes) ? kLdsRows32
                                                                                             : kLds256w8;
         const int mode1 = p.moe_type == kQwen3 ? kGateUp : kFc1;
         const long long dev_wgs = 8LL * std::max(cus_per_xcd(), 32);
+        const long long tiles_o2 = est_tiles(128) * cdiv(I, gemm_tile_cols(mode1, kLds128x256o2));
         if (p.cfg == kLds256w8 && P <= kOneTileRows * touched)
             p.cfg = touched * cdiv(I, gemm_tile_cols(mode1, kLds128)) <= 2 * dev_wgs ? kLds128 : kLds128x256o2;
-        else if (p.cfg == kLds256w8 && H <= 1024 && est_tiles(256) * cdiv(I, gemm_tile_cols(mode1, kLds256w8)) < dev_wgs)
-            p.cfg = kLds128;
+        else if (p.cfg == kLds256w8 && H <= 1024 && tiles_o2 <= 2 * dev_wgs)
+            p.cfg = tiles_o2 <= dev_wgs ? kLds128 : kLds128x256o2;
+        else if (p.cfg == kLds256w8 && P >= kTwoTileRows * touched && P < 320 * touched &&
+                 (est_tiles(128) + touched / 2) * cdiv(I, gemm_tile_cols(mode1, kLds128x256o2)) >= 2 * dev_wgs)
+            p.cfg = kLds128x256o2;
         if (p.cfg == kLdsRows32 && H > 1024 && P > 32 * touched &&
             (est_tiles(32) + touched / 2) * cdiv(I, gemm_tile_cols(mode1, kLdsRows32)) > dev_wgs &&
             touched * cdiv(I, gemm_tile_cols(mode1, kLds128)) <= dev_wgs && P <= kOneTileRows * touched)
             p.cfg = kLds128;
         // 8-bit rows that go as they are (bf16): the 256x256 kernel has that form
-        // (Qwen3-30B-A3B T=1024 / 2048 181 / 224 us against 210 / 278)
+        // (Qwen3-30B-A3B T=1024 / 2048 / 4096 179 / 223 / 382 us against 183 / 281 / 439)
         if (p.cfg == kLds128x256o2 && mx8 && p.dtype == kBF16 && H % 128 == 0) p.cfg = kLds256w8;
         if ((is_lds_cfg(g_tile_policy) && g_tile_policy != kW8Gemv) || (g_tile_policy == kDecGemv && dec_gemv_fits(p)))
             p.cfg = g_tile_policy;

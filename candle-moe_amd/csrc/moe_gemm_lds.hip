@@ -95,10 +95,10 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     constexpr int S_BYTES = W4 ? BN * 4 * SDW : 0;
     constexpr int S_INS = S_BYTES / (256 * NW);  // (one dword per lane)
     static_assert(S_INS * 256 * NW == S_BYTES, "scale DMA split");
-    static_assert(EXT == 0 || (EXT == 32 && NW == 4 && BM == 128 && WGM == 2 && NB % 2 == 0 && !ATOMIC && !W8),
+    static_assert(EXT == 0 || (EXT == 32 && NW == 4 && BM == 128 && (WGM == 1 ? W4 : NB % 2 == 0) && !ATOMIC && !W8),
                   "extended tiles");
     constexpr bool EX = EXT > 0;
-    constexpr int NX = EX ? NB / 2 : 1;     // column blocks of the extension rows per wave
+    constexpr int NX = EX ? NB / WGM : 1;   // column blocks of the extension rows per wave
     constexpr int X_INS = EX ? EXT / RPA : 1;  // DMA instructions of the extension rows (per stage)
     constexpr int XN = X_INS > NW ? X_INS / NW : 1;  // and per wave
     constexpr int X_OFF = A_BYTES + B_BYTES + S_BYTES;
@@ -753,10 +753,12 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
             }
         };
         load_a(0);
+        // the tile's first scale byte in its column's dwords: 32 columns hold K bytes, a
+        // multiple of 32, so every block's columns start alike
+        const uint32_t first = (uint32_t)lr * (uint32_t)(a.ldb / 32) + (uint32_t)(kk0 / 32);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int r = (DUAL ? (nb & 1) * SUBN + wn * (WN / 2) + (nb >> 1) * 32 : wn * WN + nb * 32) + lr;
-            const uint32_t first = (uint32_t)(nt * SUBN + r % SUBN) * (uint32_t)(a.ldb / 32) + (uint32_t)(kk0 / 32);
             if constexpr (BK >= 64) {
                 const uint64_t d = *reinterpret_cast<const uint64_t*>(sS + r * 8);
 #pragma unroll
@@ -1009,7 +1011,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
             f32x16 blk[1][NX];
 #pragma unroll
             for (int j = 0; j < NX; ++j) blk[0][j] = accx[j];
-            tile_epilogue<DT, MODE, BN, 32, NX * 32, 1, NX>(a, blk, r0 + BM, m_valid - BM, nt, 0, 2 * wn + wm, lane,
+            tile_epilogue<DT, MODE, BN, 32, NX * 32, 1, NX>(a, blk, r0 + BM, m_valid - BM, nt, 0, WGM * wn + wm, lane,
                                                             s_tok + BM, nullptr);
         }
     }
@@ -1031,7 +1033,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
 #pragma unroll
                 for (int j = 0; j < NX; ++j) blk[0][j] = accx[j];
                 const int dst[1] = {s_dst[BM + lr]};
-                rows32_epilogue<BN, 32, NX * 32, 1, NX>(a, blk, m_valid - BM, nt, 0, 2 * wn + wm, lane, dst);
+                rows32_epilogue<BN, 32, NX * 32, 1, NX>(a, blk, m_valid - BM, nt, 0, WGM * wn + wm, lane, dst);
             }
         }
         return;
@@ -1158,7 +1160,11 @@ static hipError_t launch_mx_mode(int cfg, const GemmArgs& a, hipStream_t stream)
     if (nwg_l <= 0) return hipSuccess;
     if (a.ext != 0 && ext_rows_of(cfg) != a.ext) return hipErrorInvalidValue;
     const dim3 g((unsigned)nwg_l);
-    constexpr int X = kTileExt;
+    // 128x256 tiles: K tiles of 64 in two stages (of 32 in three: Qwen3-30B-A3B
+    // T=4096 gate/up 331, down 188 us); for down the 4 waves side by side, so that a
+    // weight block is converted by one wave only: 182 -> 165 us, gate/up 286 -> 274
+    // but at half-empty tiles (T=1024), whose second wave row then has work, 121 -> 150
+    constexpr int X = kTileExt, WGM = MODE == kGateUp || MODE == kFc1 ? 2 : 1;
     switch (cfg) {
         case kLds128:
             hipLaunchKernelGGL((moe_lds_gemm<DT, 128, 128, 128, 3, 4, MODE, 2, 1, false, false, X, true>), g, dim3(256), 0,
@@ -1169,7 +1175,7 @@ static hipError_t launch_mx_mode(int cfg, const GemmArgs& a, hipStream_t stream)
                                stream, a);
             break;
         case kLds128x256o2:
-            hipLaunchKernelGGL((moe_lds_gemm<DT, 128, 256, 32, 3, 4, MODE, 2, 2, false, false, X, true>), g, dim3(256), 0,
+            hipLaunchKernelGGL((moe_lds_gemm<DT, 128, 256, 64, 2, 4, MODE, WGM, 2, false, false, X, true>), g, dim3(256), 0,
                                stream, a);
             break;
         case kLdsRows32:
