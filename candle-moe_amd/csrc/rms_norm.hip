@@ -11,9 +11,12 @@
 //     (MXFP8 of y before any rounding)
 //
 // Bound by its bytes: every element of x and r is read once and held in f32
-// registers between the sum of squares and the outputs. NT threads share a row,
-// each holding CH chunks of 8 consecutive elements (16-byte loads of 16-bit
-// rows); 4 neighbouring lanes hold a block of 32.
+// registers between the sum of squares (in f64) and the outputs. NT threads share a
+// row, each holding CH chunks of 8 consecutive elements (16-byte loads of 16-bit
+// rows); 4 neighbouring lanes hold a block of 32. bf16, all outputs: T=8191 H 4096
+// 60 us (5.1 TB/s, what a copy reaches), f16 T=1000 H 2880 without codes 6.4 us with
+// its launch, T=1 H 2048 2.1 us on the GPU (loads, two barriers' worth of
+// reduction, stores).
 #include "cm_common.hpp"
 #include "cm_internal.hpp"
 
@@ -78,15 +81,52 @@ __device__ __forceinline__ u32x2 mxfp8_codes(const float (&y)[8], uint32_t& scal
     return u32x2{(uint32_t)lo, (uint32_t)hi};
 }
 
+// 1/sqrt(mean + eps) as a sum of two f32. With it y = z * inv * w comes as a sum of
+// two as well, within 2^-40 of its value. A y rounded to f32 can fall on the middle
+// between two 8-bit codes, or on the border of two scales, and then goes the wrong
+// way (some 20 of 33 million values); rounded to odd (cut off, the last bit set
+// where anything was) it stays on its side.
+struct InvNorm {
+    float hi, lo;
+    __device__ __forceinline__ InvNorm(double sq, int H, float eps) {
+        const double m = sq * (1.0 / (double)H) + (double)eps;
+        double v;
+        if (m > 1e-30 && m < 1e30) {  // (one Newton step on the f32 value: 2^-42)
+            v = (double)__builtin_amdgcn_rsqf((float)m);
+            v = fma(0.5 * v, fma(-m * v, v, 1.0), v);
+        } else {
+            v = 1.0 / sqrt(m);
+        }
+        hi = (float)v;
+        lo = hi < INFINITY ? (float)(v - (double)hi) : 0.f;
+    }
+    // y to the nearest f32; rest: what that left out
+    __device__ __forceinline__ float times(float z, float w, float& rest) const {
+        const float p = z * hi;
+        const float e = fmaf(z, lo, fmaf(z, hi, -p));  // (|z| hi <= sqrt(H): no overflow)
+        float t = e * w;
+        t = fabsf(t) < INFINITY ? t : 0.f;
+        const float y = fmaf(p, w, t);
+        rest = fmaf(p, w, -y) + t;
+        return y;
+    }
+};
+__device__ __forceinline__ float to_odd(float y, float rest) {
+    uint32_t u = __float_as_uint(y);
+    const bool below = (__float_as_uint(rest) ^ u) >> 31;  // (nearer to zero than y)
+    if (fabsf(rest) > 0.f && fabsf(y) < INFINITY && y != 0.f) u = (u - (below ? 1u : 0u)) | 1u;
+    return __uint_as_float(u);
+}
+
 template <int NT>
-__device__ __forceinline__ float row_sum(float v, float* s_part) {
+__device__ __forceinline__ double row_sum(double v, double* s_part) {
     constexpr int IN = NT < 64 ? NT : 64;
 #pragma unroll
     for (int m = 1; m < IN; m <<= 1) v += __shfl_xor(v, m);
     if constexpr (NT > 64) {
         if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = v;
         __syncthreads();
-        v = 0.f;
+        v = 0.0;
 #pragma unroll
         for (int w = 0; w < NT / 64; ++w) v += s_part[w];
     }
@@ -96,13 +136,13 @@ __device__ __forceinline__ float row_sum(float v, float* s_part) {
 template <int DT, int NT, int CH>
 __global__ __launch_bounds__(NT > kNormThreads ? NT : kNormThreads) void rms_norm_k(NormArgs a) {
     constexpr int RPW = NT > kNormThreads ? 1 : kNormThreads / NT;  // rows per workgroup
-    __shared__ float s_part[NT > 64 ? NT / 64 : 1];
+    __shared__ double s_part[NT > 64 ? NT / 64 : 1];
     const int t = threadIdx.x % NT;
     const long long row = (long long)blockIdx.x * RPW + threadIdx.x / NT;
     if (row >= a.T) return;  // (NT > 64: one row per workgroup, all its threads stay)
     const long long base = row * (long long)a.H;
     float z[CH][8];
-    float sq = 0.f;
+    double sq = 0.0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int h = (c * NT + t) * 8;
@@ -115,21 +155,23 @@ __global__ __launch_bounds__(NT > kNormThreads ? NT : kNormThreads) void rms_nor
             for (int j = 0; j < 8; ++j) z[c][j] += r[j];
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sq = fmaf(z[c][j], z[c][j], sq);
+        for (int j = 0; j < 8; ++j) sq = fma((double)z[c][j], (double)z[c][j], sq);
     }
     sq = row_sum<NT>(sq, s_part);
-    const float inv = 1.0f / sqrtf(sq / (float)a.H + a.eps);
+    const InvNorm inv(sq, a.H, a.eps);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int h = (c * NT + t) * 8;
         if (h >= a.H) continue;
         if (a.residual_out) store8<DT>(a.residual_out, base + h, z[c]);
-        float y[8], w[8];
+        float y[8], rest[8], w[8];
         load8<DT>(a.weight, h, w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = z[c][j] * inv * w[j];
+        for (int j = 0; j < 8; ++j) y[j] = inv.times(z[c][j], w[j], rest[j]);
         if (a.out) store8<DT>(a.out, base + h, y);
         if (a.codes) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = to_odd(y[j], rest[j]);
             // (hidden sizes of 8-bit calls are multiples of 32: a block's four
             // lanes are all here)
             uint32_t s;
@@ -145,24 +187,25 @@ __global__ __launch_bounds__(NT > kNormThreads ? NT : kNormThreads) void rms_nor
 template <int DT>
 __global__ __launch_bounds__(kNormThreads) void rms_norm_any_k(NormArgs a) {
     typedef typename Elem<DT>::storage S;
-    __shared__ float s_part[kNormThreads / 64];
+    __shared__ double s_part[kNormThreads / 64];
     const long long base = (long long)blockIdx.x * a.H;
     const S* x = reinterpret_cast<const S*>(a.x) + base;
     const S* r = a.residual ? reinterpret_cast<const S*>(a.residual) + base : nullptr;
     auto at = [&](int h) { return Elem<DT>::to_f32(x[h]) + (r ? Elem<DT>::to_f32(r[h]) : 0.f); };
-    float sq = 0.f;
+    double sq = 0.0;
     for (int h = threadIdx.x; h < a.H; h += kNormThreads) {
         const float z = at(h);
-        sq = fmaf(z, z, sq);
+        sq = fma((double)z, (double)z, sq);
     }
     sq = row_sum<kNormThreads>(sq, s_part);
-    const float inv = 1.0f / sqrtf(sq / (float)a.H + a.eps);
+    const InvNorm inv(sq, a.H, a.eps);
     for (int h = threadIdx.x; h < a.H; h += kNormThreads) {
         const float z = at(h);
         if (a.residual_out) reinterpret_cast<S*>(a.residual_out)[base + h] = Elem<DT>::from_f32(z);
+        float rest;
         if (a.out)
             reinterpret_cast<S*>(a.out)[base + h] =
-                Elem<DT>::from_f32(z * inv * Elem<DT>::to_f32(reinterpret_cast<const S*>(a.weight)[h]));
+                Elem<DT>::from_f32(inv.times(z, Elem<DT>::to_f32(reinterpret_cast<const S*>(a.weight)[h]), rest));
     }
 }
 

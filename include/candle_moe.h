@@ -361,10 +361,11 @@ int candle_moe_topk_route(const void* logits, uint32_t logits_dtype, const float
  * layer (no counterpart in the reference: its callers use candle's), with the
  * 8-bit rows candle_moe_fused_moe_mxfp4 takes:
  *   z = input + residual (input where residual is NULL), residual_output = dtype(z);
- *   y = z / sqrt(mean(z^2) + eps) * weight, of z in f32; output = dtype(y);
+ *   y = z / sqrt(mean(z^2) + eps) * weight, of z in f32, the mean in f64;
+ *   output = dtype(y);
  *   codes, scales: y as MXFP8 (OCP): per 32 values along the row the byte e + 127
  *   of the least e with max|y| <= 448 * 2^e (0 for zeros, 255 where one is not
- *   finite), and the e4m3 code of y / 2^e, ties to even.
+ *   finite), and the e4m3 code of y / 2^e, ties to even, both of y to 2^-40.
  * input, residual, residual_output, output [num_tokens, hidden_dim] and weight
  * [hidden_dim] of dtype; codes u8 [num_tokens, hidden_dim], scales u8 [num_tokens,
  * hidden_dim / 32]. residual, residual_output, output may be NULL, codes and scales

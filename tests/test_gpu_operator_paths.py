@@ -69,6 +69,27 @@ def test_past_one_launch_of_rows():
     assert torch.equal(r[part], (2 * x[part].float()).to(BF))
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("T, H", [(1500, 2048), (3000, 480), (40, 16384)])
+def test_codes_are_those_of_the_exact_norm(T, H, dtype):
+    # scales and codes of the 64-bit y itself, each rounded once: a y rounded to f32
+    # on the way would change some 2 of these 3 million codes
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x, r = (torch.randn(T, H, device="cuda", generator=g).to(dtype) for _ in range(2))
+    w = (1 + 0.1 * torch.randn(H, device="cuda", generator=g)).to(dtype)
+    codes, scales = (torch.empty(T, n, dtype=torch.uint8, device="cuda") for n in (H, H // 32))
+    cm.add_rms_norm(x, w, 1e-6, residual=r, codes=codes, scales=scales)
+    z = (x.float() + r.float()).double()  # (as the kernel's z)
+    _, y = ref.norm(z, w, float(np.float32(1e-6)))
+    b = y.unflatten(-1, (-1, 32))
+    s = ref.mx_scale(b.abs().amax(-1), 448.0)
+    assert torch.equal(scales, s)
+    v = b / ref.scale_value(s).unsqueeze(-1)
+    step = torch.exp2(torch.floor(torch.log2(v.abs())).clamp(min=-6) - 3)
+    want_v = torch.round(v / step) * step
+    assert torch.equal(codes.view(torch.float8_e4m3fn).double(), want_v.flatten(-2))
+
+
 # ------------------------------------------------------------- decode of MXFP4
 @pytest.mark.parametrize("rows8", [False, True])
 @pytest.mark.parametrize("dtype", [BF, F16])
