@@ -141,7 +141,7 @@ __global__ __launch_bounds__(NT > kNormThreads ? NT : kNormThreads) void rms_nor
     const long long row = (long long)blockIdx.x * RPW + threadIdx.x / NT;
     if (row >= a.T) return;  // (NT > 64: one row per workgroup, all its threads stay)
     const long long base = row * (long long)a.H;
-    float z[CH][8];
+    float z[CH][8], w[CH][8];  // (the weights before the reduction, not behind it)
     double sq = 0.0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -151,8 +151,11 @@ __global__ __launch_bounds__(NT > kNormThreads ? NT : kNormThreads) void rms_nor
         if (a.residual) {
             float r[8];
             load8<DT>(a.residual, base + h, r);
+            load8<DT>(a.weight, h, w[c]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) z[c][j] += r[j];
+        } else {
+            load8<DT>(a.weight, h, w[c]);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) sq = fma((double)z[c][j], (double)z[c][j], sq);
@@ -164,10 +167,9 @@ __global__ __launch_bounds__(NT > kNormThreads ? NT : kNormThreads) void rms_nor
         const int h = (c * NT + t) * 8;
         if (h >= a.H) continue;
         if (a.residual_out) store8<DT>(a.residual_out, base + h, z[c]);
-        float y[8], rest[8], w[8];
-        load8<DT>(a.weight, h, w);
+        float y[8], rest[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = inv.times(z[c][j], w[j], rest[j]);
+        for (int j = 0; j < 8; ++j) y[j] = inv.times(z[c][j], w[c][j], rest[j]);
         if (a.out) store8<DT>(a.out, base + h, y);
         if (a.codes) {
 #pragma unroll
