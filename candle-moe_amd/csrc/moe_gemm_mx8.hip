@@ -9,6 +9,11 @@
 // column); the sums across K are f32. The intermediate's rounding to 16 bits, right
 // after, is larger.
 //
+// Qwen3 T=16384 gate/up: 436 us (1.89 PFLOP/s; a library product of 8192^3 in fp8
+// 3.0), on 16-bit copies of the rows 728 us. Per K tile and CU 50 KB come into LDS
+// and 160 KB of fragments go out, some 1650 cycles of its port under the 2048 of the
+// MFMAs: the two do not overlap fully.
+//
 // Tile 256 x 256, K tiles of 128, 8 waves (2 x 4), three LDS stages filled by DMA:
 // 32 KB of row codes, 16 KB of weight codes, a dword of scales per row and column
 // (the tile's four 32 k). Lane (h, r) (h = lane / 32) of a 64-k step holds, of the

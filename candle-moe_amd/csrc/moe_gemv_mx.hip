@@ -1,5 +1,7 @@
 // Decode GEMMs over MXFP4 expert weights (gfx950): few rows per touched expert, so
 // the time is the weight stream (4.25 bits a weight) and the latency around it.
+// Qwen3 T=16: gate/up 13.9 us (53.5 MB, 3.8 TB/s), down 8.9 (26.7 MB, 3.0 TB/s);
+// from 8-bit rows T=8 13.5 / 8.4; Qwen3-30B-A3B T=1 7.2 / 5.5 us (13.4 / 6.7 MB).
 //
 // As in moe_gemv_dec.hip a workgroup finds its item (touched expert, block of
 // 16 * CPL columns) and the expert's pairs itself, its 4 waves split K (gate/up:

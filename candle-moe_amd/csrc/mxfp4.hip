@@ -10,6 +10,10 @@
 // dequantize: value * 2^e, exact in f32 and bf16; in f16 it is rounded where it
 // leaves that type's range.
 // MXFP8 rows (e4m3 codes, the same scales): rows8_to dequantizes those.
+// All bound by their bytes. quantize (once per weight tensor) bf16 128 x 2048 x 768:
+// [K,N] 181 us (2.8 TB/s; neighbouring threads read neighbouring columns but write
+// 16 bytes apart), [N,K] 382 us (each thread its own 64 bytes); dequantize 123 us
+// (4.1 TB/s).
 #include <algorithm>
 
 #include "cm_common.hpp"
