@@ -24,6 +24,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -394,9 +395,10 @@ static int dec_cap() { return 2 * 8 * std::max(cus_per_xcd(), 32); }
 // pairs) 102 against 115 us.
 constexpr long long kDecDefaultPairs = 256;
 // MXFP4 weights: the decode kernels up to kMxDecPairs (steps, decode against
-// 32-row kernel: Qwen3 T=64 / 128 42 / 73 against 46 / 63 us, Qwen3-30B-A3B T=16 /
-// 32 73 / 118 against 80 / 107, H 768 I 2048 E 8 k 2 T=64 / 128 18 / 26 against 28 /
-// 27); most bytes for the 32-row kernel beyond 32 rows per touched expert.
+// 32-row kernel: Qwen3 T=32 / 64 / 96 34 / 42 / 44 against 39 / 41 / 40 us, from
+// 8-bit rows T=64 / 96 38 / 41 against 42 / 44; Qwen3-30B-A3B T=16 / 24 66 / 94
+// against 74 / 94; H 768 I 2048 E 8 k 2 T=64 / 96 19 / 20 against 28 / 28); most
+// bytes for the 32-row kernel beyond 32 rows per touched expert.
 constexpr long long kMxDecPairs = 128;
 constexpr long long kMxRows32StreamBytes = 192LL << 20;
 // 16-bit prefill batches: rows per touched expert up to which nearly every
@@ -851,7 +853,7 @@ struct Fp8Weights {
 // or 2 (blocks of 48 and 96 columns put Qwen3's 1536 and Nomic's 3072
 // columns of 8 experts into 256 items).
 // f32: 4 columns (the same 16 bytes per lane and k-row; slices even out the items).
-static int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32, int most) {
+static int dec_cpl(double groups, int N, bool trans, int ks_lim, bool f32, int most) {
     if (f32) return 4;
     if (ks_lim > 1) return 8;
     const double cus = 8.0 * std::max(cus_per_xcd(), 32);
@@ -862,7 +864,7 @@ static int dec_cpl(long long groups, int N, bool trans, int ks_lim, bool f32, in
     double best_b = -1.0;
     for (int i = 0; i < ncand; ++i) {
         if (cand[i] > most) continue;
-        const double items = (double)groups * cdiv(N, 16 * cand[i]);
+        const double items = groups * cdiv(N, 16 * cand[i]);
         const double b = items / std::ceil(items / cus);
         if (b > best_b + 1e-9) {
             best_b = b;
@@ -912,7 +914,13 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     d.rows_max = (int)std::min<long long>(p.P, p.T);
     d.cap = dec_cap();
     d.ks_lim = p.dec_ks1;
-    d.cpl = dec_cpl(d.max_groups, p.I, !nk, d.ks_lim, p.dtype == kF32,
+    // MXFP4 gate/up: blocks for the experts that T tokens of k touch on average
+    // (against min(P, E): Qwen3-30B-A3B T=2 / 6 / 12 13.3 / 25.2 / 41.6 -> 11.4 / 22.1 /
+    // 35.7 us, H 2880 I 1024 E 32 k 4 T=8 25.8 -> 22.8; down, with its short K, prefers
+    // the wider blocks of min(P, E): Qwen3-30B-A3B T=4 12.2 against 16.1 us)
+    const double touched = mx ? std::min<double>(d.max_groups, p.E * (1.0 - std::pow(std::max(0.0, 1.0 - (double)p.k / p.E), p.T)))
+                              : d.max_groups;
+    d.cpl = dec_cpl(touched, p.I, !nk, d.ks_lim, p.dtype == kF32,
                     mx ? mx_dec_cols(qwen3 ? kGateUp : kFc1, d.rows_max, p.H) : 8);
     d.nblk = cdiv(p.I, 16 * d.cpl);
     const int mode1 = qwen3 ? kGateUp : kFc1;
