@@ -400,6 +400,7 @@ constexpr long long kDecDefaultPairs = 256;
 // against 74 / 94; H 768 I 2048 E 8 k 2 T=64 / 96 19 / 20 against 28 / 28); most
 // bytes for the 32-row kernel beyond 32 rows per touched expert.
 constexpr long long kMxDecPairs = 128;
+constexpr long long kMxSumBytes = 16LL << 20;
 constexpr long long kMxRows32StreamBytes = 192LL << 20;
 // 16-bit prefill batches: rows per touched expert up to which nearly every
 // expert's rows fit one extended 128-row tile (160 rows: two standard
@@ -969,6 +970,20 @@ static int run_moe_dec(const Problem& p, const void* x, const void* gate, const 
     d2.cpl = dec_cpl(d.max_groups, p.H, qwen3 && !nk, d2.ks_lim, p.dtype == kF32,
                      mx ? mx_dec_cols(kDownRows, d.rows_max, p.I) : 8);
     d2.nblk = cdiv(p.H, 16 * d2.cpl);
+    // MXFP4: down and the token sums in one launch where the tokens share few experts
+    // or all their rows' weights are little (steps, two launches against one:
+    // Qwen3-30B-A3B T=1 / 2 / 6 / 12 14.1 / 18.8 / 38.4 / 59.5 against 13.0 / 16.2 / 31.6 /
+    // 54.0 us, Qwen3 T=1 / 3 / 4 14.4 / 20.4 / 24.3 against 13.1 / 19.8 / 24.8, H 2880
+    // I 1024 E 32 k 4 T=1 / 4 / 8 13.8 / 25.4 / 34.5 against 12.7 / 24.3 / 36.5, H 768
+    // I 2048 E 8 k 2 T=1 / 8 / 12 11.7 / 12.9 / 13.2 against 9.3 / 12.5 / 14.1)
+    if (mx && p.k <= kMxSumSlots && p.I <= kMxSumMaxK &&
+        (5.0 * (double)p.P <= 7.0 * touched || (double)p.P * p.H * p.I * 17 / 32 <= (double)kMxSumBytes)) {
+        const MxDecSum sum = {rw, out, p.T, p.k, overwrite ? 1 : 0, 0};
+        ProfScope ps(kSlotGemm2, s);
+        e = launch_mx_dec_sum(p.dtype, d2, sum, s);
+        if (e != hipSuccess) return hip_fail(e, "fused_moe decode down GEMM and row sums");
+        return CANDLE_MOE_OK;
+    }
     {
         ProfScope ps(kSlotGemm2, s);
         e = mx ? launch_mx_dec(kDownRows, p.dtype, d2, s)

@@ -369,6 +369,16 @@ constexpr int kMxDecLds = 150 * 1024;
 constexpr int kMxDecMaxK = 16384;
 int mx_dec_cols(int mode, int rows_max, int K);
 hipError_t launch_mx_dec(int mode, int dtype, const DecArgs& a, hipStream_t stream);
+// Down / fc2 over MXFP4 codes and the sum over each token's k <= kMxSumSlots slots,
+// K <= kMxSumMaxK: out [T, N] of dtype (parts: set by the launch).
+constexpr int kMxSumSlots = 16;
+constexpr int kMxSumMaxK = 4096;
+struct MxDecSum {
+    const float* w;  // [T, k]
+    void* out;
+    int T, k, overwrite, parts;
+};
+hipError_t launch_mx_dec_sum(int dtype, const DecArgs& a, const MxDecSum& s, hipStream_t stream);
 // Finishing the K slices of a decode GEMM (fixed slice order: deterministic),
 // ks = meta[0] (gate/up, fc1) or meta[1] (down, fc2), as the GEMM stored it.
 // kGateUp / kFc1 (nothing to do when ks == 1): inter[p] = dtype(act(s0 *

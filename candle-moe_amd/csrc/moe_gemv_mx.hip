@@ -1,7 +1,7 @@
 // Decode GEMMs over MXFP4 expert weights (gfx950): few rows per touched expert, so
 // the time is the weight stream (4.25 bits a weight) and the latency around it.
 // Qwen3 T=16: gate/up 13.9 us (53.5 MB, 3.8 TB/s), down 8.9 (26.7 MB, 3.0 TB/s);
-// from 8-bit rows T=8 13.5 / 8.4; Qwen3-30B-A3B T=1 7.2 / 5.5 us (13.4 / 6.7 MB).
+// from 8-bit rows T=8 13.5 / 8.4; Qwen3-30B-A3B T=1 gate/up 7.2 us (13.4 MB).
 //
 // As in moe_gemv_dec.hip a workgroup finds its item (touched expert, block of
 // 16 * CPL columns) and the expert's pairs itself, its 4 waves split K (gate/up:
@@ -294,6 +294,92 @@ __global__ __launch_bounds__(64 * kMxWaves, 2) void mx_dec_k(DecArgs a) {
     }
 }
 
+// Down / fc2 of a few tokens with the sum over a token's experts in the same launch:
+// a workgroup has 16 columns of one token, its 8 waves the token's slots (and K
+// parts of them where the slots are few). A wave streams its expert's 16 columns
+// like the kernel above, rows and scales through its own LDS (it waits for its own
+// DMA only); the MFMA's 16 rows are the one row. Then out = sum_j w_j y_j in slot
+// order, each y_j its K parts in order. No partial rows in memory and no finishing
+// launch; tokens of one expert read its weights each. T=1 down:
+// Qwen3-30B-A3B 6.0 us (two launches 5.5 + 2.8), Qwen3 5.8: trips to cold memory.
+constexpr int kSumWaves = 8;
+
+template <int DT>
+__global__ __launch_bounds__(64 * kSumWaves) void mx_dec_sum_k(DecArgs a, MxDecSum f) {
+    constexpr int RING = 8;
+    __shared__ float s_part[kMxSumSlots][16];
+    extern __shared__ __attribute__((aligned(16))) char s_dyn[];
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, li = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int t = blockIdx.y, col0 = blockIdx.x * 16;
+    const int K = a.K, kb = K / 32;
+    const int rowb = (2 * K + 1023) & ~1023, scb = (16 * kb + 1023) & ~1023;
+    char* s_row = s_dyn + wave * (rowb + scb);
+    const uint8_t* s_sc = reinterpret_cast<const uint8_t*>(s_row + rowb) + li * kb + g;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(s_row));
+    const int slot0 = wave / f.parts, part = wave - slot0 * f.parts, step = kSumWaves / f.parts;
+    const int nst = (K + 127) / 128, per = (nst + f.parts - 1) / f.parts;
+    const int lo = part * per, n = min(per, nst - lo);
+    const long long wbytes = a.strideB / 2, sbytes = a.strideB / 32;
+    const i32x4 rA = make_rsrc(a.A, a.a_bytes);
+    const uint32_t wlane = (uint32_t)(col0 + li) * (uint32_t)(K / 2) + 16u * (uint32_t)g;
+
+    for (int j = slot0; j < f.k; j += step) {
+        const int p = t * f.k + j;
+        const uint32_t e = __builtin_amdgcn_readfirstlane(a.idx[p]);
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        if (e < (uint32_t)a.E && n > 0) {
+            for (int q = 0; q < rowb >> 10; ++q) {
+                const uint32_t at = (uint32_t)q * 1024u + 16u * (uint32_t)lane;
+                dma16(rA, lds0 + (uint32_t)(q * 1024), at < 2u * (uint32_t)K ? (uint32_t)p * 2u * (uint32_t)K + at : kOob);
+            }
+            const i32x4 rs = make_rsrc(a.mx0 + e * sbytes, sbytes);
+            for (int q = 0; q < scb >> 10; ++q)
+                dma16(rs, lds0 + (uint32_t)(rowb + q * 1024),
+                      (uint32_t)col0 * (uint32_t)kb + (uint32_t)q * 1024u + 16u * (uint32_t)lane);
+            const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<char*>(reinterpret_cast<const char*>(a.B0)) + e * wbytes, 0, (int)wbytes, 0x00020000);
+            u32x4 wv[RING];
+            auto load = [&](int i, int st) {
+                const int k = (lo + st) * 128;
+                const bool in = (st < n) & (k + 32 * g < K);
+                wv[i] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? wlane + (uint32_t)(k / 2) : kOob, 0, 0);
+            };
+#pragma unroll
+            for (int i = 0; i < RING; ++i) load(i, i);
+            wait_vm<RING>();  // the row and the scales
+            for (int st0 = 0; st0 < n; st0 += RING) {
+#pragma unroll
+                for (int i = 0; i < RING; ++i) {
+                    // (steps past the last have zero codes; their k stays in the row)
+                    const int st = min(st0 + i, n - 1), k = (lo + st) * 128, kq = k / 32;
+                    const u32x4* src = reinterpret_cast<const u32x4*>(s_row + 2 * k + 64 * g);
+                    const uint32_t sb = s_sc[kq];
+                    const float sc = __uint_as_float((st0 + i < n && kq + g < kb ? sb : 127u) << 23);
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) acc = mfma16<DT>(src[m], mx4x8_to<DT>(wv[i][m], sc), acc);
+                    if (st0 + RING < n) load(i, st0 + i + RING);
+                }
+            }
+            asm volatile("" ::: "memory");  // (the LDS of the next slot: after these reads)
+        }
+        if (g == 0) s_part[j * f.parts + part][li] = acc[0];
+    }
+    __syncthreads();
+    if (tid < 16) {
+        const long long at = (long long)t * a.N + col0 + tid;
+        uint16_t* out = reinterpret_cast<uint16_t*>(f.out);
+        float s = f.overwrite ? 0.f : Elem<DT>::to_f32(out[at]);
+        for (int j = 0; j < f.k; ++j) {
+            if (a.idx[t * f.k + j] >= (uint32_t)a.E) continue;  // (a dropped pair)
+            float y = s_part[j * f.parts][tid];
+            for (int q = 1; q < f.parts; ++q) y += s_part[j * f.parts + q][tid];
+            s = fmaf(f.w[t * f.k + j], y, s);
+        }
+        out[at] = Elem<DT>::from_f32(s);
+    }
+}
+
 template <int DT, int MODE, int RB, int CPL, bool X8>
 hipError_t launch_one(const DecArgs& a, hipStream_t stream) {
     const long long nwg = (long long)a.max_groups * a.nblk;
@@ -354,6 +440,20 @@ int mx_dec_cols(int mode, int rows_max, int K) {
     // (two row blocks of 8 columns do not fit 256 registers; scales at most 32 KB)
     const int most = (mode == kGateUp ? 1 : 2) * 32768 / K;
     return std::min(rows_max > 16 ? 6 : 8, most);
+}
+
+hipError_t launch_mx_dec_sum(int dtype, const DecArgs& a, const MxDecSum& s, hipStream_t stream) {
+    MxDecSum f = s;
+    f.parts = f.k > 4 ? 1 : f.k > 2 ? 2 : f.k > 1 ? 4 : 8;
+    const int lds = kSumWaves * ((2 * a.K + 1023) / 1024 * 1024 + (a.K / 2 + 1023) / 1024 * 1024);
+    if (f.k < 1 || f.k * f.parts > kMxSumSlots || a.mx0 == nullptr || a.K % 32 || a.N % 32 || a.K > kMxSumMaxK ||
+        f.T < 1 || f.T > 65535)
+        return hipErrorInvalidValue;
+    const dim3 grid((unsigned)(a.N / 16), (unsigned)f.T), block(64 * kSumWaves);
+    if (dtype == kBF16) hipLaunchKernelGGL(mx_dec_sum_k<kBF16>, grid, block, (unsigned)lds, stream, a, f);
+    else if (dtype == kF16) hipLaunchKernelGGL(mx_dec_sum_k<kF16>, grid, block, (unsigned)lds, stream, a, f);
+    else return hipErrorInvalidValue;
+    return hipGetLastError();
 }
 
 hipError_t launch_mx_dec(int mode, int dtype, const DecArgs& a, hipStream_t stream) {

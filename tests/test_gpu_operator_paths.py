@@ -108,6 +108,27 @@ def test_decode_of_many_pairs_and_long_rows(T, H, I, E, k, dtype, rows8):
             cm.set_tile_policy(cm.TILE_AUTO)
 
 
+@pytest.mark.parametrize("moe_type", [0, 1])
+@pytest.mark.parametrize("T, H, I, E, k", [(1, 64, 96, 2, 1), (1, 256, 1536, 8, 2), (1, 32, 32, 40, 16), (2, 96, 160, 64, 9),
+                                          (1, 128, 4096, 16, 3), (1, 64, 4128, 16, 3), (1, 64, 128, 40, 17), (1, 2048, 768, 128, 8),
+                                          (3, 512, 1056, 100, 5), (9, 768, 2048, 8, 1), (12, 320, 736, 200, 10)])
+def test_a_few_tokens_with_their_sums(T, H, I, E, k, moe_type):
+    # 1 to 8 K parts of a slot, several slots of a wave, dropped pairs, both outputs
+    dt = BF if T % 2 else F16
+    s = setup(T, H, I, E, k, moe_type, dt, moe_type == 1, seed=T + I, dropped=0.0 if E == 2 else 0.2)
+    first = check_moe(s, (T + k) % 3)
+    assert torch.equal(first, check_moe(s, (T + k) % 3))
+    big = randn(T + 1, H, seed=9).to(dt).cuda()
+    before = big.clone()
+    y, far = want(s, 0)
+    run(s, 0, big[:T], accumulate=True)
+    total = before[:T].double() + y
+    ref.within(big[:T], total, far + ref.HALF[dt] * (total.abs() + far))
+    assert torch.equal(big[T:], before[T:])
+    s["idx"].fill_(E)
+    assert (run(s, 0, torch.ones(T, H, dtype=dt, device="cuda")) == 0).all()
+
+
 @pytest.mark.parametrize("tile", [cm.TILE_DEC_GEMV, cm.TILE_ROWS32, cm.TILE_LDS_128, cm.TILE_W8])
 @pytest.mark.parametrize("rows8", [False, True])
 def test_one_expert_in_every_slot(tile, rows8):
