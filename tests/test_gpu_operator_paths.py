@@ -242,3 +242,19 @@ def test_a_block_in_one_graph(T, H, I, E, k, tile):
                 assert torch.equal(caught[n], eager[n]), n
     finally:
         cm.set_tile_policy(cm.TILE_AUTO)
+
+
+@pytest.mark.parametrize("tile", [cm.TILE_DEC_GEMV, cm.TILE_ROWS32, cm.TILE_LDS_128, cm.TILE_128x256_OCC2, cm.TILE_W8])
+@pytest.mark.parametrize("T, H", [(2, 256), (40, 416)])
+def test_a_row_that_is_nan_stays_alone(T, H, tile):
+    # a scale of 255 in one row's last block, a NaN code in another's first
+    cm.set_tile_policy(tile)
+    try:
+        s = setup(T, H, 128, 4, 2, 0, BF, True, seed=3)
+        s["x_scale"][0, H // 32 - 1] = 255
+        s["x"][1, 0] = 0x7F
+        out = run(s, 0, torch.empty(T, H, dtype=BF, device="cuda"))
+        nan = torch.isnan(out)
+        assert nan[:2].all() and not nan[2:].any()
+    finally:
+        cm.set_tile_policy(cm.TILE_AUTO)
