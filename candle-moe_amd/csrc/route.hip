@@ -27,12 +27,13 @@
 //    k + 2 rounds give the k best and the next two. Where two neighbours in that
 //    order (or a group at the border of the choice) are closer than 2 tau and the
 //    grid, and not an exact tie (equal logits and biases), or a value is not
-//    finite, the row goes the exact way: about one row in 500 of f32 logits. The
+//    finite, the row goes the exact way: about one in 15000 of normal f32 logits (groups
+//    closer than 2.4e-6). The
 //    k weights come from f64 exponentials of the chosen logits, one lane each.
-//    T = 4099 / 32768 6.6 / 20.8 us, where reading the logits takes 0.9 / 7: bound by
-//    the VALU (T = 32768: 8 waves per SIMD of 1117 vector instructions each, 17 of
-//    the 20.8 us: exponentials, keys, the lanes' sorted lists, k + 2 rounds of
-//    exchanges). T = 1 of 128 experts 3.4 us.
+//    T = 4099 6.0 us (8.4 where one row goes the exact way), T = 32768 19.8, where
+//    reading the logits takes 0.9 / 7: bound by the VALU (T = 32768: 8 waves per SIMD
+//    of 989 vector instructions each, 15 us: exponentials, keys, the lanes' sorted
+//    lists, k + 2 rounds of exchanges). T = 1 of 128 experts 3.4 us.
 #include <limits.h>
 #include <math.h>
 
@@ -256,7 +257,8 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
     const int nval = grp < groups ? max(0, min(f.cells - cell, VPT)) : 0;
     const int e0 = grp * f.cells + cell;
     const S* src = reinterpret_cast<const S*>(a.logits) + row * (long long)a.E;
-    auto ours = [&](int j) { return WHOLE ? nval > 0 : j < nval; };
+    // (WHOLE: a lane without experts computes on zeros and is left out lane by lane)
+    auto ours = [&](int j) { return WHOLE || j < nval; };
 
     // scores and what the choice goes by
     float l[VPT], c[VPT], b[VPT];
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
         m = -INFINITY;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) m = ours(j) ? fmaxf(m, l[j]) : m;
-        m = group_max<LPR>(m);
+        m = group_max<LPR>(nval > 0 ? m : -INFINITY);
         float part[VPT];
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
@@ -315,7 +317,7 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
         for (int q = VPT / 2; q >= 1; q /= 2)
 #pragma unroll
             for (int j = 0; j < q; ++j) part[j] += part[j + q];
-        total = group_sum<LPR>((double)part[0]);
+        total = group_sum<LPR>(nval > 0 ? (double)part[0] : 0.0);
         const float inv = __builtin_amdgcn_rcpf((float)total);
         tau = 9e-7f * inv;
 #pragma unroll
@@ -333,7 +335,7 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
         zero = ours(j) ? fmaf(c[j], 0.f, zero) : zero;
         c[j] = ours(j) ? c[j] : -INFINITY;
     }
-    bool unsure = !(zero == 0.f);
+    bool unsure = nval > 0 && !(zero == 0.f);
 
     bool kept = nval > 0;
     if (groups > 1) {
@@ -343,6 +345,7 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
             b2 = fmaxf(b2, fminf(b1, c[j]));
             b1 = fmaxf(b1, c[j]);
         }
+        if (WHOLE && nval == 0) b1 = b2 = -INFINITY;
         if (f.lanes_log2 > 0) top2_step<1>(b1, b2);
         if (f.lanes_log2 > 1) top2_step<2>(b1, b2);
         if (f.lanes_log2 > 2) top2_step<4>(b1, b2);
@@ -381,12 +384,17 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
     tau += 3.6e-7f * fmaxf(fabsf(hi), fabsf(lo));  // roundings of c, of first and of the product
     // (f32 holds 24 bits of a grid of more)
     const uint32_t apart = (uint32_t)fminf(2.f * tau * unit, 1e9f) + (16u << (QB > 24 ? QB - 24 : 0));
+    // Experts in question lie at 1 (what is below the grid) and above, those of lanes
+    // that are not kept at 0 (v_med3 takes a NaN to the lower bound): keys below kNone
+    // are nobody's.
+    constexpr uint32_t kNone = 1u << IB;
+    const float lane_unit = kept ? unit : 0.f, lane_first = kept ? first : 0.f, lane_low = kept ? 1.f : 0.f;
     uint32_t key[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        // (the conversion takes what is below the grid, and a NaN, to 0)
-        const uint32_t q = (uint32_t)__builtin_amdgcn_fmed3f(fmaf(c[j], unit, first), 1.f, (float)((1u << QB) - 1u));
-        key[j] = kept && ours(j) ? (q << IB) | (uint32_t)(SLOTS - 1 - (sub * VPT + j)) : 0u;
+        const uint32_t q =
+            (uint32_t)__builtin_amdgcn_fmed3f(fmaf(c[j], lane_unit, lane_first), lane_low, (float)((1u << QB) - 1u));
+        key[j] = ours(j) ? (q << IB) | (uint32_t)(SLOTS - 1 - (sub * VPT + j)) : 0u;
     }
     constexpr int NL = VPT > 8 ? VPT / 8 : 1, LEN = VPT / NL;  // sorted lists per lane
 #pragma unroll
@@ -409,7 +417,7 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
     // places 0 .. k + 1, one lane each, and their scores in 64 bits
     const int slot = SLOTS - 1 - (int)(mine & (SLOTS - 1));
     const int sg = (slot / VPT) >> f.lanes_log2;
-    const bool has = sub <= a.k + 1 && mine != 0u;
+    const bool has = sub <= a.k + 1 && mine >= kNone;
     int e = has ? sg * f.cells + slot - (sg << f.lanes_log2) * VPT : INT_MAX;
     const float le = has ? Elem<DT>::to_f32(src[e]) : -INFINITY;
     const double be = has && a.bias ? (double)a.bias[e] : 0.0;
@@ -423,12 +431,12 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
     // k - 1; the order of places 0 .. k goes by their exact c (those of a softmax
     // with a bias would need the exact sum: those rows need clear places).
     const uint32_t k1 = __shfl_down(mine, 1), k2 = __shfl_down(mine, 2);
-    unsure |= sub < a.k && mine == 0u;
-    unsure |= sub == a.k - 1 && k2 != 0u && (mine >> IB) - (k2 >> IB) <= apart;
+    unsure |= sub < a.k && mine < kNone;
+    unsure |= sub == a.k - 1 && k2 >= kNone && (mine >> IB) - (k2 >> IB) <= apart;
     if (soft && a.bias) {
         const float nl = __shfl_down(le, 1);
         const double nb = __shfl_down(be, 1);
-        unsure |= sub < a.k && k1 != 0u && (mine >> IB) - (k1 >> IB) <= apart && !(le == nl && be == nb);
+        unsure |= sub < a.k && k1 >= kNone && (mine >> IB) - (k1 >> IB) <= apart && !(le == nl && be == nb);
     } else {
         const double ce = w + be;
         const double nc = __shfl_down(ce, 1);
