@@ -27,9 +27,9 @@
 //    k + 2 rounds give the k best and the next two. Where two neighbours in that
 //    order (or a group at the border of the choice) are closer than 2 tau and the
 //    grid, and not an exact tie (equal logits and biases), or a value is not
-//    finite, the row goes the exact way: about one in 15000 of normal f32 logits (groups
-//    closer than 2.4e-6). The
-//    k weights come from f64 exponentials of the chosen logits, one lane each.
+//    finite, the row goes the exact way: about one in 15000 of normal f32 logits
+//    (groups closer than 2.4e-6). The k weights come from f64 exponentials of the
+//    chosen logits, one lane each.
 //    T = 4099 6.0 us (8.4 where one row goes the exact way), T = 32768 19.8, where
 //    reading the logits takes 0.9 / 7: bound by the VALU (T = 32768: 8 waves per SIMD
 //    of 989 vector instructions each, 15 us: exponentials, keys, the lanes' sorted
