@@ -402,6 +402,7 @@ constexpr long long kDecDefaultPairs = 256;
 constexpr long long kMxDecPairs = 128;
 constexpr long long kMxSumBytes = 16LL << 20;
 constexpr long long kMxRows32StreamBytes = 192LL << 20;
+constexpr long long kMxLongBytes = 32LL << 20;
 // 16-bit prefill batches: rows per touched expert up to which nearly every
 // expert's rows fit one extended 128-row tile (160 rows: two standard
 // deviations of uniform routing above), and from which a 256-row tile often
@@ -541,7 +542,12 @@ static int check_problem(int T, int H, int I, int E, int k, int act, uint32_t mo
         // tiles that fill the device (H 768 I 2048 E 8 k 2: T=2000 67 / 85 / 84,
         // T=3000 99 / 89 / 90, T=4096 116 / 105 / 121, T=8192 203 / 162 / 164).
         const long long stream = est_tiles(32) * (p.moe_type == kQwen3 ? 3LL : 2LL) * H * I * 17 / 32;
-        p.cfg = P <= kMxDecPairs && dec_gemv_fits(p) ? kDecGemv
+        // (Long streams over 16-bit rows leave the decode kernels from 12 rows per
+        // expert on: an expert of more than 32 rows is read twice. Qwen3 T=48 / 64 39 / 42
+        // against 40 / 41 us, with skewed routing 59 / 64 against 43 / 44.)
+        const bool long_rows = !mx8 && P >= 12 * touched &&
+                               touched * (p.moe_type == kQwen3 ? 3LL : 2LL) * H * I * 17 / 32 >= kMxLongBytes;
+        p.cfg = P <= kMxDecPairs && !long_rows && dec_gemv_fits(p) ? kDecGemv
                 : P <= 32 * touched || (P <= 384 * touched && stream <= kMxRows32StreamBytes) ? kLdsRows32
                                                                                             : kLds256w8;
         const int mode1 = p.moe_type == kQwen3 ? kGateUp : kFc1;
