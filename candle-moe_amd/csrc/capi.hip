@@ -794,7 +794,8 @@ static size_t upto_bytes(const Problem& p) {
         choose_dec_slices(q);
         acc = std::max(acc, dec_part_bytes(q));
     }
-    if (!dec || forced || P > dec_pairs) {
+    // (MXFP4: large weights leave the decode kernels before dec_pairs)
+    if (!dec || forced || P > dec_pairs || (p.mx && P >= 12 * touched)) {
         const int n1 = cdiv(p.I, 64), n2 = cdiv(p.H, 64);  // (the narrowest column tile)
         o += a256((size_t)tiles * std::max(n1, n2) * 4);   // split-K counters
         if (f32) {

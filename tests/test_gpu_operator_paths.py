@@ -194,6 +194,31 @@ def test_the_binding_and_ctypes_give_the_same(monkeypatch):
         assert np.array_equal(a, b)
 
 
+def test_captures_of_smaller_batches_on_both_sides_of_the_decode_kernels():
+    H, I, E, k = 2048, 1408, 8, 2  # (37 MB of codes and scales)
+    s = setup(64, H, I, E, k, 0, BF, False, seed=2)
+    cut = {T: dict(s, **{n: s[n][:T].contiguous() for n in ("x", "rw", "idx")}) for T in (64, 56, 49, 48, 40, 9)}
+    outs = {T: torch.empty(T, H, dtype=BF, device="cuda") for T in cut}
+    cm.trim_workspaces()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run(cut[64], 0, outs[64])
+    torch.cuda.synchronize()
+    graphs = {}
+    for T in cut:
+        graphs[T] = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graphs[T], stream=side):
+            run(cut[T], 0, outs[T])
+    for T, g in graphs.items():
+        eager = run(cut[T], 0, torch.empty_like(outs[T]))
+        outs[T].zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager, outs[T]), T
+    ref.within(outs[56], *want(cut[56], 0))
+
+
 @pytest.mark.parametrize("T, H, I, E, k, tile", [(24, 512, 256, 16, 4, cm.TILE_AUTO), (300, 512, 256, 8, 2, cm.TILE_W8),
                                                 (600, 256, 128, 4, 1, cm.TILE_128x256_OCC2)])
 def test_a_block_in_one_graph(T, H, I, E, k, tile):
