@@ -124,16 +124,24 @@ __device__ __forceinline__ void route_exact_row(const RouteArgs& a, long long ro
         for (int j = 0; j < VPT; ++j) buf[lane * VPT + j] = c[j];
         wave_lds_fence();
         double b1 = -(double)INFINITY, b2 = -(double)INFINITY;
-        if (lane < a.groups) {
-            for (int q = 0; q < per; ++q) {
-                const double v = buf[lane * per + q];
+        // the lanes of a group (a power of two of them) share its experts
+        const int lanes = 64 >> (32 - __builtin_clz((unsigned)(a.groups - 1)));
+        const int g = lane / lanes, first = lane - g * lanes;
+        if (g < a.groups) {
+            for (int q = first; q < per; q += lanes) {
+                const double v = buf[g * per + q];
                 b2 = fmax(b2, fmin(b1, v));
                 b1 = fmax(b1, v);
             }
         }
+        for (int x = 1; x < lanes; x <<= 1) {
+            const double o1 = __shfl_xor(b1, x), o2 = __shfl_xor(b2, x);
+            b2 = fmax(fmin(b1, o1), fmax(b2, o2));
+            b1 = fmax(b1, o1);
+        }
         double gs = a.group_top == 1 ? b1 : b1 + b2;
         if (!(gs == gs)) gs = -(double)INFINITY;
-        int gi = lane < a.groups ? lane : INT_MAX;
+        int gi = g < a.groups && first == 0 ? g : INT_MAX;
         uint64_t keep = 0;
         for (int q = 0; q < a.topk_groups; ++q) {
             double v = gs;
