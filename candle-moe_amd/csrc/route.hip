@@ -30,8 +30,9 @@
 //    finite, the row goes the exact way: about one in 15000 of normal f32 logits
 //    (groups closer than 2.4e-6). The k weights come from f64 exponentials of the
 //    chosen logits, one lane each.
-//    T = 4099 6.0 us (8.4 where one row goes the exact way), T = 32768 19.8, where
-//    reading the logits takes 0.9 / 7: bound by the VALU (T = 32768: 8 waves per SIMD
+//    T = 4099 6.1 us, up to 11.8 where a row goes the exact way, T = 32768 16 to 21
+//    (none to four such rows), where reading the logits takes 0.9 / 7: bound by such
+//    a row's dependent steps and the VALU (T = 32768: 8 waves per SIMD
 //    of 989 vector instructions each, 15 us: exponentials, keys, the lanes' sorted
 //    lists, k + 2 rounds of exchanges). T = 1 of 128 experts 3.4 us.
 #include <limits.h>
@@ -141,18 +142,16 @@ __device__ __forceinline__ void route_exact_row(const RouteArgs& a, long long ro
         }
         double gs = a.group_top == 1 ? b1 : b1 + b2;
         if (!(gs == gs)) gs = -(double)INFINITY;
-        int gi = g < a.groups && first == 0 ? g : INT_MAX;
-        uint64_t keep = 0;
-        for (int q = 0; q < a.topk_groups; ++q) {
-            double v = gs;
-            int i = gi;
-            wave_best(v, i);
-            keep |= 1ull << i;
-            if (gi == i) gi = INT_MAX;
+        // its place among the groups, ties to the lower one
+        int place = 0;
+        for (int q = 0; q < a.groups; ++q) {
+            const double v = __shfl(gs, q * lanes);
+            place += v > gs || (v == gs && q < g);
         }
+        const uint64_t keep = __ballot(g < a.groups && first == 0 && place < a.topk_groups);
 #pragma unroll
         for (int j = 0; j < VPT; ++j)
-            if (!((keep >> ((lane * VPT + j) / per)) & 1ull)) alive &= ~(1u << j);
+            if (lane * VPT + j < a.E && !((keep >> ((lane * VPT + j) / per * lanes)) & 1ull)) alive &= ~(1u << j);
         wave_lds_fence();
     }
 
@@ -168,22 +167,18 @@ __device__ __forceinline__ void route_exact_row(const RouteArgs& a, long long ro
             }
         }
         wave_best(v, i);
-        double w = 0.0;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             if (i == lane * VPT + j) {
-                w = s[j];
+                buf[q] = s[j];
                 alive &= ~(1u << j);
             }
         }
-        w = __shfl(w, i / VPT);
-        total += w;
-        if (lane == 0) {
-            buf[q] = w;
-            a.idx[row * a.k + q] = (uint32_t)i;
-        }
+        if (lane == 0) a.idx[row * a.k + q] = (uint32_t)i;
     }
     wave_lds_fence();
+    if (a.renorm)
+        for (int q = 0; q < a.k; ++q) total += buf[q];
     for (int q = lane; q < a.k; q += 64) {
         double w = buf[q];
         if (a.renorm) w = total == 0.0 ? 0.0 : w / total;
