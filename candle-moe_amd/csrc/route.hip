@@ -391,12 +391,17 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
     // that are not kept at 0 (v_med3 takes a NaN to the lower bound): keys below kNone
     // are nobody's.
     constexpr uint32_t kNone = 1u << IB;
+    // the grid's last place that f32 holds (2^QB - 1 rounds to 2^QB where QB > 24, which
+    // the shift would take out of the key): roundings of unit and first carry the
+    // largest c past it
+    constexpr float kLast = (float)((1u << QB) - (QB > 24 ? 1u << (QB - 24) : 1u));
+    static_assert((uint32_t)kLast < (1u << QB), "the largest key fits 32 bits");
     const float lane_unit = kept ? unit : 0.f, lane_first = kept ? first : 0.f, lane_low = kept ? 1.f : 0.f;
     uint32_t key[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const uint32_t q =
-            (uint32_t)__builtin_amdgcn_fmed3f(fmaf(c[j], lane_unit, lane_first), lane_low, (float)((1u << QB) - 1u));
+            (uint32_t)__builtin_amdgcn_fmed3f(fmaf(c[j], lane_unit, lane_first), lane_low, kLast);
         key[j] = ours(j) ? (q << IB) | (uint32_t)(SLOTS - 1 - (sub * VPT + j)) : 0u;
     }
     constexpr int NL = VPT > 8 ? VPT / 8 : 1, LEN = VPT / NL;  // sorted lists per lane
