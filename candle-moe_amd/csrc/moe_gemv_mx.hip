@@ -348,19 +348,35 @@ __global__ __launch_bounds__(64 * kSumWaves) void mx_dec_sum_k(DecArgs a, MxDecS
 #pragma unroll
             for (int i = 0; i < RING; ++i) load(i, i);
             wait_vm<RING>();  // the row and the scales
-            for (int st0 = 0; st0 < n; st0 += RING) {
+            auto compute = [&](int i, int st) {
+                const int k = (lo + st) * 128, kq = k / 32;
+                const u32x4* src = reinterpret_cast<const u32x4*>(s_row + 2 * k + 64 * g);
+                const uint32_t sb = s_sc[kq];
+                // past K the codes are zeros, and a foreign scale could be a NaN
+                const float sc = __uint_as_float((kq + g < kb ? sb : 127u) << 23);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) acc = mfma16<DT>(src[m], mx4x8_to<DT>(wv[i][m], sc), acc);
+            };
+            // full rounds, then what is left, as above: a step past the last would
+            // multiply the row by zeros, which an infinity in it turns into a NaN
+            int st = 0;
+            for (; st + RING < n; st += RING) {
 #pragma unroll
                 for (int i = 0; i < RING; ++i) {
-                    // (steps past the last have zero codes; their k stays in the row)
-                    const int st = min(st0 + i, n - 1), k = (lo + st) * 128, kq = k / 32;
-                    const u32x4* src = reinterpret_cast<const u32x4*>(s_row + 2 * k + 64 * g);
-                    const uint32_t sb = s_sc[kq];
-                    const float sc = __uint_as_float((st0 + i < n && kq + g < kb ? sb : 127u) << 23);
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) acc = mfma16<DT>(src[m], mx4x8_to<DT>(wv[i][m], sc), acc);
-                    if (st0 + RING < n) load(i, st0 + i + RING);
+                    compute(i, st + i);
+                    load(i, st + i + RING);
                 }
             }
+            auto rest = [&](auto self, auto ic) -> void {
+                constexpr int i = decltype(ic)::value;
+                if constexpr (i < RING) {
+                    if (st + i < n) {
+                        compute(i, st + i);
+                        self(self, std::integral_constant<int, i + 1>{});
+                    }
+                }
+            };
+            rest(rest, std::integral_constant<int, 0>{});
             asm volatile("" ::: "memory");  // (the LDS of the next slot: after these reads)
         }
         if (g == 0) s_part[j * f.parts + part][li] = acc[0];
