@@ -320,8 +320,15 @@ __global__ __launch_bounds__(64 * kRouteWaves, LPR * VPT <= 256 ? 5 : 4) void ro
         for (int q = VPT / 2; q >= 1; q /= 2)
 #pragma unroll
             for (int j = 0; j < q; ++j) part[j] += part[j + q];
-        total = group_sum<LPR>(nval > 0 ? (double)part[0] : 0.0);
-        const float inv = __builtin_amdgcn_rcpf((float)total);
+        const double near = group_sum<LPR>(nval > 0 ? (double)part[0] : 0.0);
+        const float inv = __builtin_amdgcn_rcpf((float)near);
+        if (!a.renorm) {
+            // weights are divided by the sum: of 64-bit exponentials, as in the exact form
+            double sum = 0.0;
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) sum += ours(j) ? exp((double)l[j] - (double)m) : 0.0;
+            total = group_sum<LPR>(nval > 0 ? sum : 0.0);
+        }
         tau = 9e-7f * inv;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) c[j] = fmaf(c[j], inv, b[j]);
