@@ -85,9 +85,12 @@ __device__ __forceinline__ u32x2 mxfp8_codes(const float (&y)[8], uint32_t& scal
 // two as well, within 2^-40 of its value. A y rounded to f32 can fall on the middle
 // between two 8-bit codes, or on the border of two scales, and then goes the wrong
 // way (some 20 of 33 million values); rounded to odd (cut off, the last bit set
-// where anything was) it stays on its side.
+// where anything was) it stays on its side. Where 1/sqrt(mean + eps) or its second
+// part leaves f32's normal range (rows near the ends of it), the two hold it times
+// 2^-sh, and z goes in times 2^sh.
 struct InvNorm {
     float hi, lo;
+    int sh = 0;
     __device__ __forceinline__ InvNorm(double sq, int H, float eps) {
         const double m = sq * (1.0 / (double)H) + (double)eps;
         double v;
@@ -96,12 +99,14 @@ struct InvNorm {
             v = fma(0.5 * v, fma(-m * v, v, 1.0), v);
         } else {
             v = 1.0 / sqrt(m);
+            if (v > 0.0 && v < (double)INFINITY) v = frexp(v, &sh);
         }
         hi = (float)v;
         lo = hi < INFINITY ? (float)(v - (double)hi) : 0.f;
     }
     // y to the nearest f32; rest: what that left out
     __device__ __forceinline__ float times(float z, float w, float& rest) const {
+        z = ldexpf(z, sh);
         const float p = z * hi;
         const float e = fmaf(z, lo, fmaf(z, hi, -p));  // (|z| hi <= sqrt(H): no overflow)
         float t = e * w;
