@@ -59,6 +59,8 @@ struct NormArgs {
     float eps;
 };
 constexpr int kNormMaxRows = 1 << 21;  // of one launch (up to 1024 threads per row)
+constexpr int kNormThreads = 256;      // of a workgroup, for rows of any size
+constexpr int kNormMaxHidden = 0x7fffffff - kNormThreads;  // (its loops step past a row by as much)
 hipError_t launch_add_rms_norm(const NormArgs& a, int dtype, hipStream_t stream);
 
 // -------------------------------------------------------------- grouping

@@ -131,7 +131,9 @@ int candle_moe_add_rms_norm(const void* input, const void* residual, const void*
     cm::clear_error();
     const int T = num_tokens, H = hidden_dim;
     if (T < 0) return cm::set_error(CANDLE_MOE_ERR_INVALID, "add_rms_norm: num_tokens must be >= 0 (got %d)", T);
-    if (H < 1) return cm::set_error(CANDLE_MOE_ERR_INVALID, "add_rms_norm: hidden_dim must be >= 1 (got %d)", H);
+    if (H < 1 || H > cm::kNormMaxHidden)
+        return cm::set_error(CANDLE_MOE_ERR_INVALID, "add_rms_norm: hidden_dim must be in [1, %d] (got %d)",
+                             cm::kNormMaxHidden, H);
     if (dtype > 2) return cm::set_error(CANDLE_MOE_ERR_INVALID, "add_rms_norm: dtype must be 0, 1 or 2 (got %u)", dtype);
     if (!(eps >= 0.0f)) return cm::set_error(CANDLE_MOE_ERR_INVALID, "add_rms_norm: eps must be >= 0 (got %g)", (double)eps);
     if (!codes != !scales)

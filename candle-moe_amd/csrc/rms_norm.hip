@@ -24,8 +24,6 @@ namespace cm {
 
 namespace {
 
-constexpr int kNormThreads = 256;  // per workgroup: 256 / NT rows
-
 template <int DT>
 __device__ __forceinline__ void load8(const void* base, long long at, float (&v)[8]) {
     if constexpr (DT == kF32) {
@@ -140,7 +138,7 @@ __device__ __forceinline__ double row_sum(double v, double* s_part) {
 
 template <int DT, int NT, int CH>
 __global__ __launch_bounds__(NT > kNormThreads ? NT : kNormThreads) void rms_norm_k(NormArgs a) {
-    constexpr int RPW = NT > kNormThreads ? 1 : kNormThreads / NT;  // rows per workgroup
+    constexpr int RPW = NT > kNormThreads ? 1 : kNormThreads / NT;  // rows per workgroup (of 256 threads)
     __shared__ double s_part[NT > 64 ? NT / 64 : 1];
     const int t = threadIdx.x % NT;
     const long long row = (long long)blockIdx.x * RPW + threadIdx.x / NT;

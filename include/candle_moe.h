@@ -371,7 +371,8 @@ int candle_moe_topk_route(const void* logits, uint32_t logits_dtype, const float
  * hidden_dim / 32]. residual, residual_output, output may be NULL, codes and scales
  * both; output or codes must be given. residual_output may be residual, and
  * output or residual_output may be input; no other overlap. The 8-bit form needs
- * hidden_dim a multiple of 32, at most 32768, and 16-byte aligned tensors. */
+ * hidden_dim a multiple of 32, at most 32768, and 16-byte aligned tensors; without
+ * it hidden_dim is at most 2^31 - 257. */
 int candle_moe_add_rms_norm(const void* input, const void* residual, const void* weight, void* residual_output,
                             void* output, void* codes, void* scales, int num_tokens, int hidden_dim, float eps,
                             uint32_t dtype, void* stream);
