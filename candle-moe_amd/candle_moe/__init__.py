@@ -539,6 +539,13 @@ def _require(who: str, device, want) -> None:
             raise CandleMoeError(CANDLE_MOE_ERR_INVALID, f"{who}: {name} {problem}")
 
 
+def _int32(who: str, **values) -> None:
+    """Each a whole number that the C entry points' ints hold (ctypes would cut it)."""
+    for name, v in values.items():
+        if not -(1 << 31) <= int(v) < 1 << 31:
+            raise CandleMoeError(CANDLE_MOE_ERR_INVALID, f"{who}: {name} must fit 32 bits, got {v}")
+
+
 def _launch_on(t, who: str, call) -> None:
     """check(call(stream)) with t's device current and its current stream."""
     import torch
@@ -585,6 +592,8 @@ def topk_route(logits, topk_weight, topk_indices, token_expert_indices, bias=Non
     if bias is not None:
         want.append(("bias", bias, (E,), (torch.float32,)))
     _require("topk_route", logits.device, want)
+    _int32("topk_route", num_tokens=T, num_experts=E, topk=tk[1], num_groups=num_groups, topk_groups=topk_groups,
+           group_top=group_top)
     _launch_on(logits, "topk_route", lambda s: lib().candle_moe_topk_route(
         _ptr(logits), _torch_dtype_code(logits), _ptr(bias), _ptr(topk_weight), _ptr(topk_indices),
         _ptr(token_expert_indices), E, T, tk[1], code, int(num_groups), int(topk_groups), int(group_top),
@@ -617,6 +626,7 @@ def add_rms_norm(input, weight, eps: float, residual=None, residual_output=None,
     if codes is not None or scales is not None:
         want += [("codes", codes, (T, H), (torch.uint8,)), ("scales", scales, (T, H // 32), (torch.uint8,))]
     _require("add_rms_norm", input.device, want)
+    _int32("add_rms_norm", num_tokens=T, hidden_dim=H)
     _launch_on(input, "add_rms_norm", lambda s: lib().candle_moe_add_rms_norm(
         _ptr(input), _ptr(residual), _ptr(weight), _ptr(residual_output), _ptr(output), _ptr(codes), _ptr(scales), T, H,
         float(eps), _torch_dtype_code(input), s))
@@ -634,6 +644,7 @@ def quantize_mxfp4(weights, input_kn: bool = True):
     E = weights.shape[0]
     K, N = (weights.shape[1], weights.shape[2]) if input_kn else (weights.shape[2], weights.shape[1])
     code = _torch_dtype_code(weights)
+    _int32("quantize_mxfp4", num_experts=E, k_dim=K, n_dim=N)
     codes = torch.empty((E, N, K // 2), dtype=torch.uint8, device=weights.device)
     scales = torch.empty((E, N, K // 32), dtype=torch.uint8, device=weights.device)
     _launch_on(weights, "quantize_mxfp4", lambda s: lib().candle_moe_quantize_mxfp4(
@@ -651,6 +662,7 @@ def dequantize_mxfp4(codes, scales, dtype):
     E, N, K = codes.shape[0], codes.shape[1], codes.shape[2] * 2
     _require("dequantize_mxfp4", codes.device, [("codes", codes, (E, N, K // 2), (torch.uint8,)),
                                                 ("scales", scales, (E, N, K // 32), (torch.uint8,))])
+    _int32("dequantize_mxfp4", num_experts=E, n_dim=N, k_dim=K)
     out = torch.empty((E, N, K), dtype=dtype, device=codes.device)
     code = _torch_dtype_code(out)
     _launch_on(codes, "dequantize_mxfp4", lambda s: lib().candle_moe_dequantize_mxfp4(
@@ -703,6 +715,8 @@ def fused_moe_mxfp4(input, gate_q, up_q, down_q, gate_scale, up_scale, down_scal
     else:
         want.append(("input", input, (T, H), () if output is None else (output.dtype,)))
     _require("fused_moe_mxfp4", input.device, want)
+    _int32("fused_moe_mxfp4", num_tokens=T, hidden_dim=H, intermediate_dim=I, num_experts=E, top_k=top_k,
+           activation=activation, moe_type=moe_type)
     _launch_on(input, "fused_moe_mxfp4", lambda s: lib().candle_moe_fused_moe_mxfp4(
         _ptr(input), _ptr(input_scale), _ptr(gate_q), _ptr(up_q), _ptr(down_q), _ptr(gate_scale), _ptr(up_scale),
         _ptr(down_scale), _ptr(routing_weights), _ptr(expert_indices), _ptr(output), T, H, I, E, int(top_k),
