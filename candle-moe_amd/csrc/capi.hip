@@ -197,7 +197,13 @@ constexpr double kSetMinRowBytes = 256.0 * 1024 * 1024;
 // it the down GEMM adds into the f32 [T, H] accumulator with atomics instead
 // (k*H*2 bytes per token against H*4), which bounds the workspace of shapes
 // whose expert sets are too many for the expert-set path (large k and E).
+// (MXFP4 calls, whose rows are f32 on every kernel, go in pieces of whole tokens
+// whose rows stay within it.)
 constexpr double kRowsMaxBytes = 2.0 * 1024 * 1024 * 1024;
+static int mx_piece_tokens(int H, int k) {
+    const long long n = (long long)(kRowsMaxBytes / (4.0 * H * k));
+    return (int)std::max<long long>(1, n >= 256 ? n / 256 * 256 : n);
+}
 // fp8 weights: most pairs for the register-operand decode kernel (kW8Gemv;
 // its workgroups re-stream an expert's weights per 32-row tile like the
 // 32-row kernel's, without that kernel's LDS stages and split-K fixup).
@@ -814,6 +820,7 @@ static size_t upto_bytes(const Problem& p) {
                 // f32 pair rows on every kernel, until the expert sets take over
                 double t = p.T;
                 if (p.set_path && g_combine_policy == 0) t = std::min(t, std::ceil(p.set_from));
+                t = std::min(t, (double)mx_piece_tokens(p.H, p.k));
                 acc = std::max(acc, (size_t)(t * p.k * p.H * 4.0));
                 if (p.mx8) o += a256((size_t)p.T * p.H * 2);
             }
@@ -1392,8 +1399,11 @@ int fused_moe_impl(const void* x, const void* gate, const void* up, const void* 
     Problem p;
     auto a16 = [](const void* q) { return ((uintptr_t)q & 15) == 0; };
     const bool aligned16 = a16(x) && a16(gate) && a16(up) && a16(down);
-    int rc = check_problem(T, H, I, E, k, act, moe_type, dtype, p, aligned16, a16(out), f8 != nullptr, packed, true,
-                           mx != nullptr, mx && mx->x_s);
+    auto problem = [&](int tokens, Problem& q) {
+        return check_problem(tokens, H, I, E, k, act, moe_type, dtype, q, aligned16, a16(out), f8 != nullptr, packed, true,
+                             mx != nullptr, mx && mx->x_s);
+    };
+    int rc = problem(T, p);
     if (rc) return rc;
     rc = check_ptrs(p, x, gate, up, down, rw, idx, out);
     if (rc) return rc;
@@ -1422,18 +1432,34 @@ int fused_moe_impl(const void* x, const void* gate, const void* up, const void* 
     if (w)
         for (int i = 0; i < 4; ++i)
             if (std::equal(layer, layer + 8, w->served[i].layer)) slot = i;
+    // MXFP4 batches whose pair rows pass kRowsMaxBytes: pieces, one after the other
+    // over one workspace, the first the largest
+    const bool pieces = mx && !p.set_path && p.cfg != kDecGemv && T > mx_piece_tokens(H, k);
+    const int piece = pieces ? mx_piece_tokens(H, k) : T, last = T - (T - 1) / piece * piece;
+    Problem q = p, r = p;  // of a whole piece, of the last
+    if (pieces && ((rc = problem(piece, q)) || (rc = problem(last, r)))) return rc;
+    const size_t need = pieces ? std::max(make_layout(q).total, make_layout(r).total) : L.total;
     const bool served = slot >= 0 && T <= w->served[slot].T;
-    const size_t full = served ? L.total : upto_bytes(p);
-    w = owned_ws_locked(dev, s, L.total, full, e);
+    const size_t full = served ? need : std::max(need, upto_bytes(q));
+    w = owned_ws_locked(dev, s, need, full, e);
     // (without memory for the reserve: not asked for again in every call)
     if (w && !served && (w->bytes >= full || !is_capturing(s))) {
         if (slot < 0) slot = w->next++ & 3;
         std::copy(layer, layer + 8, w->served[slot].layer);
         w->served[slot].T = T;
     }
-    if (!w) return ws_fail("fused_moe", L.total, e);
-    return run_moe(p, x, gate, up, down, reinterpret_cast<const float*>(rw), reinterpret_cast<const uint32_t*>(idx),
-                   out, overwrite, reinterpret_cast<char*>(w->ptr), s, f8, true, mx);
+    if (!w) return ws_fail("fused_moe", need, e);
+    if (!pieces)
+        return run_moe(p, x, gate, up, down, reinterpret_cast<const float*>(rw), reinterpret_cast<const uint32_t*>(idx),
+                       out, overwrite, reinterpret_cast<char*>(w->ptr), s, f8, true, mx);
+    for (long long t = 0; t < T && rc == CANDLE_MOE_OK; t += piece) {
+        MxWeights m = *mx;
+        if (m.x_s) m.x_s += t * (H / 32);
+        rc = run_moe(t + piece <= T ? q : r, reinterpret_cast<const char*>(x) + t * H * (m.x_s ? 1 : 2), gate, up, down,
+                     reinterpret_cast<const float*>(rw) + t * k, reinterpret_cast<const uint32_t*>(idx) + t * k,
+                     reinterpret_cast<char*>(out) + t * H * 2, overwrite, reinterpret_cast<char*>(w->ptr), s, f8, true, &m);
+    }
+    return rc;
 }
 
 // ----------------------------------------------- fused MoE without allocation

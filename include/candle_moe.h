@@ -407,7 +407,9 @@ int candle_moe_dequantize_mxfp4(const void* codes, const void* scales, int num_e
  * output = result. hidden_dim and intermediate_dim multiples of 32; input, codes,
  * weight scales and output 16-byte aligned (input_scale anywhere, 4-byte aligned
  * for the products as they are). The workspace is the library's, as fused_moe's
- * (one call of the largest size before capturing serves every smaller one).
+ * (one call of the largest size before capturing serves every smaller one). It
+ * holds at most 2 GiB of pair rows (f32, 4 * top-k * hidden_dim bytes a token):
+ * larger batches go through it in pieces of whole tokens, one after the other.
  * Kernels (candle_moe_set_tile_policy 18, 12, 5, 14, 7): decode up to 128 pairs (large
  * weights: fewer than 12 16-bit rows per expert),
  * 32-row tiles while an expert has at most 32 rows or the streamed codes stay
