@@ -152,6 +152,8 @@ def lib() -> ctypes.CDLL:
         L.candle_moe_fused_moe_path.restype = i32
         L.candle_moe_fused_moe_path_ex.argtypes = [i32] * 5 + [u32, u32]
         L.candle_moe_fused_moe_path_ex.restype = i32
+        L.candle_moe_fused_moe_mxfp4_path.argtypes = [i32] * 5 + [u32, u32, i32]
+        L.candle_moe_fused_moe_mxfp4_path.restype = i32
         L.candle_moe_profile_begin.argtypes = []
         L.candle_moe_profile_begin.restype = i32
         L.candle_moe_profile_begin_slots.argtypes = [u32]
@@ -859,9 +861,29 @@ def fused_moe_tile(num_tokens, hidden_dim, intermediate_dim, num_experts, top_k,
     return 0 if k < 0 else _TILE_ROWS[k]
 
 
+def _mxfp4_path_code(num_tokens, hidden_dim, intermediate_dim, num_experts, top_k, dtype_code, moe_type, rows8):
+    return lib().candle_moe_fused_moe_mxfp4_path(num_tokens, hidden_dim, intermediate_dim, num_experts, top_k, dtype_code,
+                                                 moe_type, 1 if rows8 else 0)
+
+
+def fused_moe_mxfp4_path(num_tokens, hidden_dim, intermediate_dim, num_experts, top_k, dtype_code, moe_type=0,
+                         rows8=False) -> str:
+    """Name of the path fused_moe_mxfp4 takes for these sizes under the current policy."""
+    code = _mxfp4_path_code(num_tokens, hidden_dim, intermediate_dim, num_experts, top_k, dtype_code, moe_type, rows8)
+    return PATH_NAMES[code if code < 0 else code & 3]
+
+
+def fused_moe_mxfp4_kernel(num_tokens, hidden_dim, intermediate_dim, num_experts, top_k, dtype_code, moe_type=0,
+                           rows8=False) -> int:
+    """GEMM kernel code (TILE_*) fused_moe_mxfp4 uses for these sizes (-1 if invalid)."""
+    code = _mxfp4_path_code(num_tokens, hidden_dim, intermediate_dim, num_experts, top_k, dtype_code, moe_type, rows8)
+    return -1 if code < 0 else (code >> 2) & 0x3f
+
+
 __all__ = [
     "Activation", "FusedMoE", "apply_topk_softmax_inplace", "CandleMoeError", "lib", "describe", "spec",
     "validate_topk_softmax", "version", "LIB_PATH", "set_combine_policy", "fused_moe_path",
     "set_tile_policy", "fused_moe_tile", "fused_moe_kernel", "quantize_fp8", "dequantize_fp8", "fused_moe_fp8",
     "topk_route", "add_rms_norm", "quantize_mxfp4", "dequantize_mxfp4", "fused_moe_mxfp4",
+    "fused_moe_mxfp4_path", "fused_moe_mxfp4_kernel",
 ]

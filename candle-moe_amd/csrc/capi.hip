@@ -1844,6 +1844,15 @@ int candle_moe_fused_moe_path(int num_tokens, int hidden_dim, int intermediate_d
     return c < 0 ? c : (c & 0xff);
 }
 
+int candle_moe_fused_moe_mxfp4_path(int num_tokens, int hidden_dim, int intermediate_dim, int num_experts,
+                                    int num_selected_experts, uint32_t dtype, uint32_t moe_type, int rows8) {
+    cm::Problem p;
+    if (dtype > 1 || cm::check_problem(num_tokens, hidden_dim, intermediate_dim, num_experts, num_selected_experts, 0,
+                                       moe_type, dtype, p, true, true, false, false, true, true, rows8 != 0))
+        return -1;
+    return (p.set_path ? 2 : 1) | (p.cfg << 2) | (p.rows_path ? (1 << 8) : 0);
+}
+
 int candle_moe_profile_begin(void) {
     std::lock_guard<std::mutex> lk(cm::g_prof_mu);
     cm::g_prof_on = true;

@@ -225,6 +225,10 @@ int candle_moe_fused_moe_path(int num_tokens, int hidden_dim, int intermediate_d
  * into an accumulator and a finalize pass). */
 int candle_moe_fused_moe_path_ex(int num_tokens, int hidden_dim, int intermediate_dim, int num_experts,
                                  int num_selected_experts, uint32_t dtype, uint32_t moe_type);
+/* The same for candle_moe_fused_moe_mxfp4, dtype 0 or 1, rows8: MXFP8 rows
+ * (16-byte aligned tensors). */
+int candle_moe_fused_moe_mxfp4_path(int num_tokens, int hidden_dim, int intermediate_dim, int num_experts,
+                                    int num_selected_experts, uint32_t dtype, uint32_t moe_type, int rows8);
 
 /* Router GEMM fused with topk-softmax (no counterpart symbol in the
  * reference; its callers compute the logits with a separate candle matmul,
