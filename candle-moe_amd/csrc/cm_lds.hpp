@@ -97,7 +97,8 @@ __device__ __forceinline__ int a_swz(int r, int c) {
 // chunks (every four rows take another order of them).
 template <int KCH>
 __device__ __forceinline__ int w4_swz(int r, int c) {
-    return KCH == 4 ? (c ^ (r >> 2)) & 3 : KCH == 2 ? c ^ ((r >> 3) & 1) : c;
+    static_assert(KCH == 4 || KCH == 2, "K tiles of 128 or 64");
+    return KCH == 4 ? (c ^ (r >> 2)) & 3 : c ^ ((r >> 3) & 1);
 }
 
 // [K,N] sub-tile rows of BCH 16-byte chunks: chunk c of k-row r is stored at

@@ -50,7 +50,7 @@ using namespace lds;
 // longer, which the fewer tiles repaid only here and there (Qwen3 T=4096 203 /
 // 136 -> 213 / 122, Nomic T=8191 112 / 80 -> 115 / 79 us).
 // W4: MXFP4 weights ([N,K/2] codes, [N,K/32] scale bytes per expert). A B row of a
-// stage is BK / 2 bytes of codes, and a column's scales come as the one or two
+// stage is BK / 2 bytes of codes, and a column's scales come as the two
 // aligned dwords that hold the tile's bytes (rows of K / 32 bytes start anywhere).
 // The products take the k of a tile in another order: lane half h holds the KSTEPS
 // chunks of 8 from h * KSTEPS on, so that its codes of the whole tile are one LDS
@@ -83,7 +83,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     constexpr bool ROWS = (MODE == kDownRows || MODE == kFc2Rows);
     constexpr bool ATOMIC = (MODE == kDown || MODE == kFc2);
     constexpr bool SWAP = !ATOMIC;
-    static_assert(BK == 32 || BK == 64 || (W4 && BK == 128), "BK");
+    static_assert(W4 ? BK == 64 || BK == 128 : BK == 32 || BK == 64, "BK");
     constexpr int ACH = BK / 8;            // 16-byte chunks per K-contiguous row
     constexpr int AROW = BK * 2;           // bytes per K-contiguous row
     constexpr int RPA = 1024 / AROW;       // K-contiguous rows per DMA instruction
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
     constexpr int KCH = KROW / 16;
     constexpr int KRPI = 1024 / KROW;  // n-rows of codes per DMA instruction
     constexpr int B_BYTES = W8 || W4 ? BN * KROW : BN * AROW;
-    constexpr int SDW = BK == 32 ? 1 : 2;  // W4: scale dwords per column and stage
+    constexpr int SDW = 2;  // W4: scale dwords per column and stage
     constexpr int S_BYTES = W4 ? BN * 4 * SDW : 0;
     constexpr int S_INS = S_BYTES / (256 * NW);  // (one dword per lane)
     static_assert(S_INS * 256 * NW == S_BYTES, "scale DMA split");
@@ -763,25 +763,17 @@ __global__ __launch_bounds__(64 * NW, OCC) void moe_lds_gemm(GemmArgs a) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int r = (DUAL ? (nb & 1) * SUBN + wn * (WN / 2) + (nb >> 1) * 32 : wn * WN + nb * 32) + lr;
-            if constexpr (BK >= 64) {
-                const uint64_t d = *reinterpret_cast<const uint64_t*>(sS + r * 8);
+            const uint64_t d = *reinterpret_cast<const uint64_t*>(sS + r * 8);
 #pragma unroll
-                for (int h = 0; h < GRP; ++h) {
-                    const int gr = GRP * lh + h;  // 32 k of the tile
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(sB + r * KROW + w4_swz<KCH>(r, gr) * 16);
+            for (int h = 0; h < GRP; ++h) {
+                const int gr = GRP * lh + h;  // 32 k of the tile
+                const u32x4 v = *reinterpret_cast<const u32x4*>(sB + r * KROW + w4_swz<KCH>(r, gr) * 16);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) braw[nb][(4 * h + q) % KSTEPS] = v[q];
-                    uint32_t e = (uint32_t)(d >> (8u * ((first & 3u) + (uint32_t)gr))) & 255u;
-                    // (past K: the codes are zeros, a foreign scale could be a NaN)
-                    if (kk0 + 32 * gr >= klim) e = 127u;
-                    sc[nb][h] = __uint_as_float(e << 23);
-                }
-            } else {
-                const u32x2 v = *reinterpret_cast<const u32x2*>(sB + r * KROW + lh * 8);
-                braw[nb][0] = v[0];
-                braw[nb][KSTEPS - 1] = v[1];
-                const uint32_t d = *reinterpret_cast<const uint32_t*>(sS + r * 4);
-                sc[nb][0] = __uint_as_float(((d >> (8u * (first & 3u))) & 255u) << 23);
+                for (int q = 0; q < 4; ++q) braw[nb][(4 * h + q) % KSTEPS] = v[q];
+                uint32_t e = (uint32_t)(d >> (8u * ((first & 3u) + (uint32_t)gr))) & 255u;
+                // (past K: the codes are zeros, a foreign scale could be a NaN)
+                if (kk0 + 32 * gr >= klim) e = 127u;
+                sc[nb][h] = __uint_as_float(e << 23);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
