@@ -169,8 +169,8 @@ __device__ __forceinline__ u32x4 fp8x8_to(const u32x2& v) {
 // bytes) times their scale as the MFMA operand of the activation dtype: the
 // gfx950 scaled conversions take the power of two as an f32 of that exponent
 // byte, 0 as 2^-127 and 255 as NaN, and round to nearest even where the dtype
-// does not hold the product (f16 only), as dequantize_mxfp4 does (checked for
-// every scale and code).
+// does not hold the product (weights: f16 only; rows also below bf16's least step), as
+// dequantize_mxfp4 does (tests/test_gpu_mxfp4_conversions.py: every scale and code).
 template <int DT>
 __device__ __forceinline__ u32x4 mx4x8_to(uint32_t v, float scale) {
     u32x4 r;

@@ -301,7 +301,7 @@ __global__ __launch_bounds__(64 * kMxWaves, 2) void mx_dec_k(DecArgs a) {
 // DMA only); the MFMA's 16 rows are the one row. Then out = sum_j w_j y_j in slot
 // order, each y_j its K parts in order. No partial rows in memory and no finishing
 // launch; tokens of one expert read its weights each. T=1 down:
-// Qwen3-30B-A3B 6.0 us (two launches 5.5 + 2.8), Qwen3 5.8: trips to cold memory.
+// Qwen3-30B-A3B 6.4 us (two launches 5.5 + 2.8), Qwen3 5.5: trips to cold memory.
 constexpr int kSumWaves = 8;
 
 template <int DT>

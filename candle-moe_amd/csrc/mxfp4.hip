@@ -7,8 +7,9 @@
 // quantize: e is the least with max|w| <= 6 * 2^e over the 32 (no value is cut
 // off), 0 as the byte for 32 zeros, 255 where a weight is not finite; w / 2^e, an
 // exact division, goes to the nearest e2m1, ties to the even code.
-// dequantize: value * 2^e, exact in f32 and bf16; in f16 it is rounded where it
-// leaves that type's range.
+// dequantize: value * 2^e, exact in f32 and bf16 (an infinity from 2^128 on, to
+// which weights past 3.5 * 2^126 go); in f16 it is rounded where it leaves that type's
+// range.
 // MXFP8 rows (e4m3 codes, the same scales): rows8_to dequantizes those.
 // All bound by their bytes. quantize (once per weight tensor) bf16 128 x 2048 x 768:
 // [K,N] 181 us (2.8 TB/s; neighbouring threads read neighbouring columns but write

@@ -15,7 +15,7 @@
 // row, each holding CH chunks of 8 consecutive elements (16-byte loads of 16-bit
 // rows); 4 neighbouring lanes hold a block of 32. bf16, all outputs: T=8191 H 4096
 // 60 us (5.1 TB/s, what a copy reaches), f16 T=1000 H 2880 without codes 6.4 us with
-// its launch, T=1 H 2048 2.1 us on the GPU (loads, two barriers' worth of
+// its launch, T=1 H 2048 2.7 us on the GPU (loads, two barriers' worth of
 // reduction, stores).
 #include "cm_common.hpp"
 #include "cm_internal.hpp"
@@ -80,7 +80,7 @@ __device__ __forceinline__ u32x2 mxfp8_codes(const float (&y)[8], uint32_t& scal
 }
 
 // 1/sqrt(mean + eps) as a sum of two f32. With it y = z * inv * w comes as a sum of
-// two as well, within 2^-40 of its value. A y rounded to f32 can fall on the middle
+// two as well, within 2^-40 of its value (a y in f32's normal range). A y rounded to f32 can fall on the middle
 // between two 8-bit codes, or on the border of two scales, and then goes the wrong
 // way (some 20 of 33 million values); rounded to odd (cut off, the last bit set
 // where anything was) it stays on its side. Where 1/sqrt(mean + eps) or its second

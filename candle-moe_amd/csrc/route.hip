@@ -7,10 +7,12 @@
 //   the `topk_groups` best groups, then the k best c in them, ties to the lower index
 //   w_j = s at the chosen, / their sum (renormalize), * scale
 //
-// Scores are 64-bit: the choice is the one the definition makes in exact
-// arithmetic unless two c differ by less than 1e-15, whatever the biases. A NaN
+// Scores are 64-bit and c is rounded to 64 bits once: the choice is the one of exact
+// arithmetic where two c differ by more than a few of their roundings, 2^-52 *
+// max(1, |c|) (with a bias of 100 scores closer than 1.4e-14 tie). A NaN
 // counts as -infinity in the choice; logits of -infinity have score 0, also
-// where a row has no others (then every weight is 0).
+// where a row has no others (then every weight is 0). Weights are 64-bit values
+// rounded to f32 once, in both forms of a row.
 //
 // Two forms of a row:
 //
@@ -29,12 +31,19 @@
 //    grid, and not an exact tie (equal logits and biases), or a value is not
 //    finite, the row goes the exact way: about one in 15000 of normal f32 logits
 //    (groups closer than 2.4e-6). The k weights come from f64 exponentials of the
-//    chosen logits, one lane each.
-//    T = 4099 6.1 us, up to 11.8 where a row goes the exact way, T = 32768 16 to 21
+//    chosen logits, one lane each; where a softmax is not renormalised they are
+//    divided by the row's sum of f64 exponentials (T = 32768: bf16 logits of 128
+//    experts 15.4 -> 18.0 us, f32 of 256 13.4 -> 20).
+//    T = 4099 6.1 us, up to 11.8 where a row goes the exact way, T = 32768 16 to 22
 //    (none to four such rows), where reading the logits takes 0.9 / 7: bound by such
 //    a row's dependent steps and the VALU (T = 32768: 8 waves per SIMD
 //    of 989 vector instructions each, 15 us: exponentials, keys, the lanes' sorted
-//    lists, k + 2 rounds of exchanges). T = 1 of 128 experts 3.4 us.
+//    lists, k + 2 rounds of exchanges). T = 1 of 128 experts 3.4 us. bf16 logits of
+//    128 experts, softmax, T = 4099 / 32768 10 / 15 us, where reading takes 0.3 / 2.2.
+//    Rows whose experts tie at the border of the choice, like a batch's padding rows of
+//    equal logits without a bias, all go the exact way, one after the other in their
+//    wave: T = 32768, 256 experts in 8 groups, the last eighth of the rows 47 us, every
+//    row 99; 128 experts, softmax, 33 / 68.
 #include <limits.h>
 #include <math.h>
 

@@ -348,7 +348,8 @@ int candle_moe_fused_moe_fp8(const void* input, const void* gate_q, const void* 
  *   groups, then the topk largest c in them are chosen, ties to the lower index;
  *   topk_weight = s at the chosen (descending c), divided by their sum where
  *   renormalize is set, times scale. The bias is in the choice alone.
- * Scores and choice in 64 bits, weights rounded to f32 once. A NaN counts as
+ * Scores and c in 64 bits (c rounded to them once: what differs by less than 2^-52 *
+ * max(1, |c|) or so ties or goes either way), weights rounded to f32 once. A NaN counts as
  * -infinity in the choice and stays a NaN in its weight; a logit of -infinity has
  * score 0, and where all chosen have score 0 the weights are 0 (not 0 / 0).
  *   logits [num_tokens, num_experts] of logits_dtype, 1 <= num_experts <= 1024;
@@ -369,7 +370,8 @@ int candle_moe_topk_route(const void* logits, uint32_t logits_dtype, const float
  *   output = dtype(y);
  *   codes, scales: y as MXFP8 (OCP): per 32 values along the row the byte e + 127
  *   of the least e with max|y| <= 448 * 2^e (0 for zeros, 255 where one is not
- *   finite), and the e4m3 code of y / 2^e, ties to even, both of y to 2^-40.
+ *   finite), and the e4m3 code of y / 2^e, ties to even, both of y to 2^-40
+ *   (where y is a normal f32).
  * input, residual, residual_output, output [num_tokens, hidden_dim] and weight
  * [hidden_dim] of dtype; codes u8 [num_tokens, hidden_dim], scales u8 [num_tokens,
  * hidden_dim / 32]. residual, residual_output, output may be NULL, codes and scales
@@ -393,7 +395,8 @@ int candle_moe_add_rms_norm(const void* input, const void* residual, const void*
 int candle_moe_quantize_mxfp4(const void* weights, uint32_t dtype, int num_experts, int k_dim, int n_dim, int input_kn,
                               void* codes, void* scales, void* stream);
 /* out [E][N][K] of dtype = dtype(value * 2^(s - 127)), the weights the MoE below
- * multiplies by: exact in f32 and bf16, in f16 rounded outside its range. */
+ * multiplies by: exact in f32 and bf16 (infinite from 2^128 on), in f16 rounded
+ * outside its range. */
 int candle_moe_dequantize_mxfp4(const void* codes, const void* scales, int num_experts, int n_dim, int k_dim, void* out,
                                 uint32_t dtype, void* stream);
 /* MoE over 4-bit weights, shapes as candle_moe_fused_moe_fp8's: Qwen3 (moe_type
@@ -401,9 +404,13 @@ int candle_moe_dequantize_mxfp4(const void* codes, const void* scales, int num_e
  * gate_q = fc1 [E][I][H], up_q = fc2 [E][H][I], down_q and down_scale unused.
  * input [num_tokens, hidden_dim] of dtype (f16, bf16) with input_scale NULL, or
  * the MXFP8 codes of candle_moe_add_rms_norm with their scales [num_tokens,
- * hidden_dim / 32] in input_scale, counted as dtype(value) (exact in bf16).
+ * hidden_dim / 32] in input_scale, counted as dtype(value) (exact in bf16
+ * from 2^-133 on).
  * f32 accumulation; the intermediate is rounded to dtype, a token's rows of its
- * experts are summed unrounded, in slot order. On the 256x256 kernel bf16 calls
+ * experts are summed unrounded, in slot order. Where large batches go by expert sets
+ * (candle_moe_fused_moe_mxfp4_path 2) the routing weight is multiplied into the
+ * intermediate before that rounding, and one f32 sum runs over the token's experts in
+ * ascending order. On the 256x256 kernel bf16 calls
  * whose hidden_dim is a multiple of 128 multiply 8-bit rows as they are: the
  * matrix instruction then aligns the 64 products of a step to the largest, up to
  * 2^-12 of the sum of their magnitudes off (2^-16 typically), which rows and
